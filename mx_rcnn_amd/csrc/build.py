@@ -83,6 +83,8 @@ def build(force=False, jobs=None, debug=False, verbose=False):
     hipcc = os.path.join(ROCM, 'bin', 'hipcc')
     opt = ['-O0', '-g'] if debug else ['-O3']
     hip_flags = opt + ['--offload-arch=%s' % ARCH, '-fPIC', '-std=c++17', '-ffp-contract=off',
+                       # no packed fp32 instructions: some of their forms have given wrong results on gfx950
+                       '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
                        '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, '-I', HERE, '-I', os.path.join(HERE, 'hip')]
     if os.environ.get('MXR_SYNC_DEBUG'):
         hip_flags.append('-DMXR_SYNC_DEBUG=1')
