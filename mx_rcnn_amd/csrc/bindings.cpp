@@ -2,6 +2,7 @@
 // outputs through the PyTorch caching allocator, launch on the current HIP stream.  All
 // launches are graph-capturable (no host sync, no allocation inside the launchers).
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -17,6 +18,7 @@
 
 #include "host_ops.h"
 #include "kernels.h"
+#include "matrix_ops.h"
 
 // a rejected launch (e.g. an LDS request over budget) must raise here, not leave the outputs
 // uninitialised for a later gather to fault on
@@ -644,6 +646,212 @@ void sgd_momentum(Tensor w, Tensor mom, const Tensor& grad, const Tensor& lr, do
   mxr::sgd_momentum(w.data_ptr<float>(), mom.data_ptr<float>(), grad.data_ptr(), is_bf16(grad), w.numel(),
                     lr.data_ptr<float>(), (float)momentum, (float)wd, (float)rescale, (float)clip, wb, cur_stream(),
                     x2_plane, planes == 3 ? 1 : 0, zp, zb);
+}
+
+// ---- Newton-Schulz orthogonalisation, Muon update (newton_schulz.hip) --------------------
+static int ns_code(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, what,
+              ": fp32, bf16 or fp16, not ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2;
+}
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Matrices {element offset, rows, cols} -> launches: groups of equal shape (in order of first appearance), at most
+// kNsMaxMats matrices, kNsMaxGroups shapes and 8 GiB of workspace each.
+static void ns_dispatch(const std::vector<std::array<int64_t, 3>>& mats, const mxr::NsUpdate& u, int64_t steps,
+                        const at::TensorOptions& o) {
+  size_t at = 0;
+  while (at < mats.size()) {
+    std::vector<std::pair<int64_t, int64_t>> shapes;
+    size_t end = at;
+    int64_t held = 0;  // workspace of the matrices so far: at most 8 GiB, or one matrix
+    for (; end < mats.size() && end - at < (size_t)mxr::kNsMaxMats; ++end) {
+      const std::pair<int64_t, int64_t> s{mats[end][1], mats[end][2]};
+      mxr::NsGroup one = {};
+      one.count = 1;
+      one.rows = (int)s.first;
+      one.cols = (int)s.second;
+      mxr::ns_shape(one);
+      held += mxr::ns_ws_elements(one) * 2;
+      if (end > at && held > ((int64_t)8 << 30)) break;
+      if (std::find(shapes.begin(), shapes.end(), s) == shapes.end()) {
+        if (shapes.size() == (size_t)mxr::kNsMaxGroups) break;
+        shapes.push_back(s);
+      }
+    }
+    std::vector<mxr::NsGroup> groups;
+    std::vector<int64_t> off;
+    int64_t ws = 0;
+    for (const auto& s : shapes) {
+      mxr::NsGroup g = {};
+      g.rows = (int)s.first;
+      g.cols = (int)s.second;
+      for (size_t k = at; k < end; ++k)
+        if (mats[k][1] == s.first && mats[k][2] == s.second) {
+          off.push_back(mats[k][0]);
+          ++g.count;
+        }
+      mxr::ns_shape(g);
+      ws += mxr::ns_ws_elements(g);
+      groups.push_back(g);
+    }
+    Tensor buf = at::empty({ws}, o.dtype(at::kHalf));
+    Tensor part = at::empty({(int64_t)off.size() * mxr::kNsParts}, o.dtype(at::kDouble));
+    mxr::ns_run(groups.data(), (int)groups.size(), off.data(), (int)off.size(), u, (int)steps,
+                reinterpret_cast<uint16_t*>(buf.data_ptr()), part.data_ptr<double>(), cur_stream());
+    LAUNCH_CHECK("newton_schulz");
+    at = end;
+  }
+}
+
+static void ns_check_shape(int64_t rows, int64_t cols) {
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  TORCH_CHECK(rows >= 1 && cols >= 1, "newton_schulz: empty matrix");
+  TORCH_CHECK(m <= 16384 && n <= (1 << 20), "newton_schulz: a matrix of ", rows, " x ", cols,
+              " (the smaller size may be 16384, the larger 1048576)");
+}
+
+// (b, r, c) contiguous -> its matrices orthogonalised, same type
+Tensor ns_orthogonalize(const Tensor& g, int64_t steps, double eps) {
+  CHECK_DEV(g); CHECK_CONTIG(g);
+  TORCH_CHECK(g.dim() == 3, "orthogonalize: (b, r, c)");
+  TORCH_CHECK(steps >= 1 && steps <= 16, "orthogonalize: 1 to 16 steps");
+  TORCH_CHECK(eps > 0, "orthogonalize: eps must be positive");
+  DevGuard guard(g.device());
+  mxr::NsUpdate u = {};
+  u.code = u.out_code = ns_code(g, "orthogonalize");
+  Tensor out = at::empty_like(g);
+  if (g.numel() == 0) return out;
+  ns_check_shape(g.size(1), g.size(2));
+  u.grad = g.data_ptr();
+  u.out = out.data_ptr();
+  u.rescale = 1.f;
+  u.eps = eps;
+  u.vec = aligned16(u.grad) && aligned16(u.out);
+  std::vector<std::array<int64_t, 3>> mats;
+  for (int64_t b = 0; b < g.size(0); ++b) mats.push_back({b * g.size(1) * g.size(2), g.size(1), g.size(2)});
+  ns_dispatch(mats, u, steps, g.options());
+  return out;
+}
+
+void muon_update(Tensor w, Tensor mom, const Tensor& grad, const std::vector<std::array<int64_t, 3>>& mats,
+                 const Tensor& lr, double momentum, double wd, double rescale, double clip, bool nesterov,
+                 int64_t steps, double eps, c10::optional<Tensor> w_bf16, int64_t planes, c10::optional<Tensor> zero,
+                 int64_t plane_stride) {
+  CHECK_DEV(w); CHECK_F32(w); CHECK_CONTIG(w); CHECK_DEV(mom); CHECK_F32(mom); CHECK_CONTIG(mom);
+  CHECK_DEV(grad); CHECK_CONTIG(grad); CHECK_DEV(lr); CHECK_F32(lr);
+  TORCH_CHECK(w.numel() == mom.numel() && w.numel() == grad.numel(), "muon_update: size mismatch");
+  TORCH_CHECK(mom.device() == w.device() && grad.device() == w.device() && lr.device() == w.device(),
+              "muon_update: tensors on different devices");
+  TORCH_CHECK(lr.numel() == 1, "muon_update: lr is one element");
+  TORCH_CHECK(steps >= 1 && steps <= 16, "muon_update: 1 to 16 steps");
+  TORCH_CHECK(eps > 0, "muon_update: eps must be positive");
+  std::vector<std::pair<int64_t, int64_t>> spans;
+  for (const auto& m : mats) {
+    ns_check_shape(m[1], m[2]);
+    TORCH_CHECK(m[0] >= 0 && m[0] + m[1] * m[2] <= w.numel(), "muon_update: matrix at ", m[0], " (", m[1], " x ", m[2],
+                ") reaches outside the buffer of ", w.numel());
+    spans.push_back({m[0], m[0] + m[1] * m[2]});
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t k = 1; k < spans.size(); ++k)
+    TORCH_CHECK(spans[k - 1].second <= spans[k].first, "muon_update: overlapping matrices");
+  mxr::NsUpdate u = {};
+  u.code = ns_code(grad, "muon_update gradient");
+  if (w_bf16.has_value() && w_bf16->defined()) {
+    // the layouts of sgd_momentum: one bf16 copy, or `planes` planes of the multi-plane modes
+    const int64_t n = w.numel(), stride = planes > 1 ? (plane_stride > 0 ? plane_stride : w_bf16->numel() / planes) : 0;
+    TORCH_CHECK(w_bf16->scalar_type() == at::kBFloat16 && w_bf16->is_contiguous() && w_bf16->device() == w.device() &&
+                    planes >= 1 && planes <= 3 && (planes == 1 || stride >= n) &&
+                    w_bf16->numel() >= (planes - 1) * stride + n,
+                "w_bf16 must be contiguous bf16 of `planes` planes of >= numel elements");
+    u.shadow = w_bf16->data_ptr();
+    u.shadow_code = planes == 1 ? 1 : planes == 2 ? mxr::kShadowX2 : mxr::kShadowX3;
+    u.shadow_plane = stride;
+  }
+  if (zero.has_value() && zero->defined()) {
+    TORCH_CHECK(zero->is_contiguous() && zero->numel() == w.numel() && zero->device() == w.device() &&
+                    (zero->scalar_type() == at::kFloat || zero->scalar_type() == at::kBFloat16),
+                "zero: contiguous fp32 / bf16 of numel elements");
+    u.zero = zero->data_ptr();
+    u.zero_code = is_bf16(*zero);
+  }
+  if (mats.empty()) return;
+  DevGuard g(w.device());
+  u.grad = grad.data_ptr();
+  u.mom = mom.data_ptr<float>();
+  u.out = u.w = w.data_ptr<float>();
+  u.lr = lr.data_ptr<float>();
+  u.mu = (float)momentum;
+  u.wd = (float)wd;
+  u.rescale = (float)rescale;
+  u.clip = (float)clip;
+  u.nesterov = nesterov;
+  u.eps = eps;
+  u.vec = aligned16(u.grad) && aligned16(u.mom) && aligned16(u.w) && aligned16(u.shadow) && u.shadow_plane % 4 == 0;
+  ns_dispatch(mats, u, steps, w.options());
+}
+
+// ---- 8-bit rows and products (int8_gemm.hip) ----------------------------------------------
+std::vector<Tensor> quantize_rows(const Tensor& x) {
+  CHECK_DEV(x);
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "quantize_rows: (M, K) with K contiguous");
+  const int code = ns_code(x, "quantize_rows");
+  TORCH_CHECK(x.size(1) <= INT32_MAX && x.size(0) <= INT32_MAX, "quantize_rows: too large");
+  DevGuard g(x.device());
+  Tensor q = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kChar));
+  Tensor s = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  if (x.size(0) > 0)
+    mxr::quantize_rows(x.data_ptr(), code, x.size(0), x.stride(0), (int)x.size(1), q.data_ptr<int8_t>(),
+                       s.data_ptr<float>(), cur_stream());
+  LAUNCH_CHECK("quantize_rows");
+  return {q, s};
+}
+
+Tensor int8_matmul(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, c10::optional<Tensor> bias,
+                   bool relu, int64_t code) {
+  CHECK_DEV(x); CHECK_DEV(w);
+  for (auto* t : {&x, &w})
+    TORCH_CHECK(t->scalar_type() == at::kChar && t->dim() == 2 && (t->stride(1) == 1 || t->size(1) <= 1),
+                "int8_matmul: operands are int8 (rows, K) with K contiguous");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(w.size(1) == K, "int8_matmul: K differs: ", K, " and ", w.size(1));
+  TORCH_CHECK(K <= 131071, "int8_matmul: K = ", K, " (int32 sums are exact up to 131071)");
+  TORCH_CHECK(M <= (1 << 24) && N <= (1 << 24), "int8_matmul: more than 2^24 rows");
+  const auto vec = [&](const Tensor& t, int64_t n, const char* what) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous() &&
+                    t.device() == x.device(),
+                "int8_matmul: ", what, " must be contiguous fp32 (", n, ",) on the operands' device");
+  };
+  vec(xs, M, "xs");
+  vec(ws, N, "ws");
+  TORCH_CHECK(w.device() == x.device(), "int8_matmul: operands on different devices");
+  mxr::Int8Args a = {};
+  if (bias.has_value() && bias->defined()) {
+    vec(*bias, N, "bias");
+    a.bias = bias->data_ptr<float>();
+  }
+  TORCH_CHECK(code >= 0 && code <= 2, "int8_matmul: output type");
+  DevGuard g(x.device());
+  Tensor y = at::empty({M, N}, x.options().dtype(code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf));
+  if (M == 0 || N == 0) return y;
+  a.x = x.data_ptr<int8_t>();
+  a.w = w.data_ptr<int8_t>();
+  a.ldx = x.stride(0);
+  a.ldw = w.stride(0);
+  a.xs = xs.data_ptr<float>();
+  a.ws = ws.data_ptr<float>();
+  a.y = y.data_ptr();
+  a.M = M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.code = (int)code;
+  a.relu = relu;
+  const int64_t bytes = mxr::int8_matmul_ws(a);
+  Tensor ws_buf = at::empty({bytes}, x.options().dtype(at::kByte));
+  mxr::int8_matmul(a, ws_buf.data_ptr(), cur_stream());
+  LAUNCH_CHECK("int8_matmul");
+  return y;
 }
 
 // ---- BN + ReLU -------------------------------------------------------------------------
@@ -2389,6 +2597,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("prev_out") = py::none(), py::arg("bnb_part") = py::none(), py::arg("x2") = 0,
         py::arg("w_plane") = 0, py::arg("bt") = false, py::arg("rmask") = py::none(), py::arg("rmask_scale") = 1.0);
   m.def("wgrad_reduce_run", &wgrad_reduce_run, py::arg("slab"), py::arg("out"));
+  m.def("ns_orthogonalize", &ns_orthogonalize, py::arg("g"), py::arg("steps"), py::arg("eps"));
+  m.def("muon_update", &muon_update, py::arg("w"), py::arg("mom"), py::arg("grad"), py::arg("mats"), py::arg("lr"),
+        py::arg("momentum"), py::arg("wd"), py::arg("rescale"), py::arg("clip"), py::arg("nesterov"), py::arg("steps"),
+        py::arg("eps"), py::arg("w_bf16"), py::arg("planes"), py::arg("zero"), py::arg("plane_stride"));
+  m.def("quantize_rows", &quantize_rows, py::arg("x"));
+  m.def("int8_matmul", &int8_matmul, py::arg("x"), py::arg("xs"), py::arg("w"), py::arg("ws"), py::arg("bias"),
+        py::arg("relu"), py::arg("code"));
   m.def("head_bwd", &head_bwd, py::arg("x"), py::arg("dys"), py::arg("ws"), py::arg("dws"), py::arg("dw_acc"),
         py::arg("dbs"), py::arg("db_acc"), py::arg("need_dx"), py::arg("relu_mask"), py::arg("x2") = 0,
         py::arg("w_planes") = std::vector<int64_t>(), py::arg("mask_scale") = 1.0);

@@ -1,0 +1,445 @@
+// Newton-Schulz orthogonalisation of weight-shaped matrices, and the Muon update built on it.
+//
+// For G (r x c), X0 = G / (|G|_F + eps), turned so that X is m x n with m <= n; a step is
+//   A = X X^T,  P = a I + b A + c A^2,  X <- P X        (a, b, c) = (3.4445, -4.7750, 2.0315).
+// P is a polynomial of A, so consecutive steps stay in the small dimension: X_{k+1} = P_k X_k gives
+// A_{k+1} = P_k A_k P_k, and X_k = P_{k-1} .. P_0 X_0 = Q X_0.  All of A, P, Q, P A commute and are
+// symmetric, so every m x m product computes the tiles on and above the diagonal and mirrors them.  Steps
+// are gathered by twos (5 = 2 + 2 + 1), after which A is formed from X anew: 9 n m^2 + 11 m^3 operations
+// for five steps against 15 n m^2 + 5 m^3 step by step.  Longer groups would be cheaper and lose: A holds
+// sigma^2, so what rounding does to the smallest directions is magnified by the square of the gain (3.44 per
+// step).  Measured on gradient-like matrices (a few strong directions over noise), error against 64 bits over that
+// of the plain recurrence in fp32: by twos 0.3 to 1.7, 3 + 2 up to 10, all five in one up to 30 and more.
+//
+// Operands are fp16 pairs (22 bits, tile_nt.h).  Single fp16 or bf16 operands were found 1e-3 to 3e-1 off: a
+// rounding of X in a small singular direction grows with that direction, up to 485 times.  fp16 holds
+// 22 bits in two planes only near the top of its range, so every buffer carries the largest power-of-two
+// scale that its spectral norm allows below 65504: X and A 2^15 (|X| <= 1.2025, |A| and |P A| <= 1.446), P and Q
+// 2^12 (|Q| <= 3.4445^2 = 11.9).
+//
+// Every m x m product is made exactly symmetric (its lower half is the mirrored upper half): the commuting of A, P
+// and Q is what the gathering rests on, and antisymmetric rounding left in them was found up to 100
+// times larger in the result (2 x 3 matrices, 1e-4).
+//
+// One launch runs a product of every matrix of the call: a block finds its matrix among the groups of
+// equal shape that the launch carries by value (no tables in memory, so a call can be captured).
+#include "tile_nt.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mxr {
+namespace {
+
+constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
+constexpr float kNsX = 32768.f, kNsP = 4096.f;  // scales of X and A, of P and Q
+
+struct NsArgs {
+  NsGroup g[kNsMaxGroups];
+  int64_t off[kNsMaxMats];  // element offset of each matrix in the flat buffers
+  int ng;
+  uint16_t* ws;
+  double* part;  // partial sums of squares: kNsParts per matrix
+};
+
+enum NsSlot { kA, kT, kP0, kP1, kQ, kSlots };
+
+// The group of work item `id` (prefix sums over groups) -> the item's number within the group.
+__device__ __forceinline__ int ns_find(const NsArgs& p, int& id, int NsGroup::*start) {
+  int k = 0;
+  while (k + 1 < p.ng && id >= p.g[k + 1].*start) ++k;
+  id -= p.g[k].*start;
+  return k;
+}
+
+__device__ __forceinline__ int64_t ns_stride(const NsGroup& g) {
+  return 6 * (int64_t)g.mp * g.np + 2 * kSlots * (int64_t)g.mp * g.mp;
+}
+// planes of matrix mi of group g: X (mp x np), its transpose in two versions (np x mp), m x m slots
+__device__ __forceinline__ uint16_t* ns_x(const NsArgs& p, const NsGroup& g, int mi) {
+  return p.ws + g.ws + mi * ns_stride(g);
+}
+__device__ __forceinline__ uint16_t* ns_xt(const NsArgs& p, const NsGroup& g, int mi, int ver) {
+  return ns_x(p, g, mi) + (2 + 2 * ver) * (int64_t)g.mp * g.np;
+}
+__device__ __forceinline__ uint16_t* ns_sq(const NsArgs& p, const NsGroup& g, int mi, int slot) {
+  return ns_x(p, g, mi) + 6 * (int64_t)g.mp * g.np + slot * 2 * (int64_t)g.mp * g.mp;
+}
+
+__device__ __forceinline__ void split_f16(float v, uint16_t& hi, uint16_t& lo) {
+  hi = f32_to_f16(v);
+  lo = f32_to_f16(v - f16_to_f32(hi));
+}
+
+// ---- the values that are orthogonalised ---------------------------------------------------------
+// u = G, or for the update g' = clip(rescale g), mom' = mu mom + g', u = g' + mu mom' (nesterov) or mom'
+__device__ __forceinline__ float ns_grad(const NsUpdate& u, int64_t i) {
+  float g = ld(u.grad, i, u.code) * u.rescale;
+  if (u.clip > 0.f) g = fminf(fmaxf(g, -u.clip), u.clip);
+  return g;
+}
+
+__device__ __forceinline__ void ns_ld4(const void* p, int64_t i, int code, bool vec, int n, float v[4]) {
+  if (vec) {
+    ld4c(p, i, code, 0, v);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = k < n ? ld(p, i + k, code) : 0.f;
+}
+
+// Pass 1: momentum, and the partial sums of u^2 (fp64: no overflow, no order dependence worth naming).
+// A matrix is cut into kNsParts runs of equal length (a multiple of 1024 elements).
+__global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs p, NsUpdate u) {
+  int id = blockIdx.x;
+  const int k = ns_find(p, id, &NsGroup::ew);
+  const NsGroup& g = p.g[k];
+  const int mi = id / g.parts, part = id % g.parts;
+  const int64_t n = (int64_t)g.rows * g.cols, off = p.off[g.first + mi];
+  const int64_t lo = (int64_t)part * g.run, hi = min(n, lo + g.run);
+  const bool vec = off % 4 == 0 && u.vec;
+  double s = 0.0;
+  for (int64_t i = lo + threadIdx.x * 4; i < hi; i += 1024) {
+    const int cnt = (int)min((int64_t)4, hi - i);
+    float v[4];
+    ns_ld4(u.grad, off + i, u.code, vec && cnt == 4, cnt, v);
+    if (u.mom != nullptr) {
+      float m[4];
+      ns_ld4(u.mom, off + i, 0, vec && cnt == 4, cnt, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float gv = v[e] * u.rescale;
+        if (u.clip > 0.f) gv = fminf(fmaxf(gv, -u.clip), u.clip);
+        m[e] = u.mu * m[e] + gv;
+        v[e] = u.nesterov ? gv + u.mu * m[e] : m[e];
+      }
+      if (vec && cnt == 4) *reinterpret_cast<float4*>(u.mom + off + i) = make_float4(m[0], m[1], m[2], m[3]);
+      else
+        for (int e = 0; e < cnt; ++e) u.mom[off + i + e] = m[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += e < cnt ? (double)v[e] * (double)v[e] : 0.0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  __shared__ double red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) p.part[(int64_t)(g.first + mi) * kNsParts + part] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// Pass 2: X = u / (|u| + eps) and its transpose, as scaled fp16 pairs with zeroed padding; 64 x 64
+// elements per block, turned in LDS.  Clears the gradient it consumed when asked to.
+__global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
+  int id = blockIdx.x;
+  const int k = ns_find(p, id, &NsGroup::init);
+  const NsGroup& g = p.g[k];
+  const int rt = (g.tall ? g.np : g.mp) / 64, ct = (g.tall ? g.mp : g.np) / 64;
+  const int mi = id / (rt * ct), t = id % (rt * ct), r0 = t / ct * 64, c0 = t % ct * 64;
+  const int64_t off = p.off[g.first + mi];
+  const int tid = threadIdx.x;
+  // the norm, from the partial sums in a fixed order
+  double s = 0.0;
+  const double* part = p.part + (int64_t)(g.first + mi) * kNsParts;
+  for (int i = tid; i < g.parts; i += 256) s += part[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  __shared__ double red[4];
+  __shared__ float tile[64][65];
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();
+  const double f = (double)kNsX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + u.eps);
+  const int lr = tid >> 4, lc = (tid & 15) * 4;
+  // elements as they lie in memory: 4 columns of rows lr, lr + 16, ..
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = r0 + lr + 16 * q, c = c0 + lc;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int cnt = r < g.rows ? max(0, min(4, g.cols - c)) : 0;
+    if (cnt > 0) {
+      const int64_t i = off + (int64_t)r * g.cols + c;
+      const bool vec = u.vec && i % 4 == 0 && cnt == 4;
+      ns_ld4(u.grad, i, u.code, vec, cnt, v);
+      if (u.mom != nullptr) {
+        float m[4];
+        ns_ld4(u.mom, i, 0, vec, cnt, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float gv = v[e] * u.rescale;
+          if (u.clip > 0.f) gv = fminf(fmaxf(gv, -u.clip), u.clip);
+          v[e] = u.nesterov ? gv + u.mu * m[e] : m[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = e < cnt ? (float)((double)v[e] * f) : 0.f;
+      if (u.zero != nullptr)
+        for (int e = 0; e < cnt; ++e) st(u.zero, i + e, 0.f, u.zero_code);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[lr + 16 * q][lc + e] = v[e];
+  }
+  __syncthreads();
+  const int64_t plane = (int64_t)g.mp * g.np;
+  uint16_t* same = g.tall ? ns_xt(p, g, mi, 0) : ns_x(p, g, mi);   // laid out as in memory
+  uint16_t* turn = g.tall ? ns_x(p, g, mi) : ns_xt(p, g, mi, 0);
+  const int lds_ = g.tall ? g.mp : g.np, ldt = g.tall ? g.np : g.mp;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int a = lr + 16 * q;
+    uint16_t h[4], l[4], ht[4], lt[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      split_f16(tile[a][lc + e], h[e], l[e]);
+      split_f16(tile[lc + e][a], ht[e], lt[e]);
+    }
+    uint16_t* d = same + (int64_t)(r0 + a) * lds_ + c0 + lc;
+    *reinterpret_cast<ushort4*>(d) = make_ushort4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(l[0], l[1], l[2], l[3]);
+    d = turn + (int64_t)(c0 + a) * ldt + r0 + lc;
+    *reinterpret_cast<ushort4*>(d) = make_ushort4(ht[0], ht[1], ht[2], ht[3]);
+    *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(lt[0], lt[1], lt[2], lt[3]);
+  }
+}
+
+// ---- products -----------------------------------------------------------------------------------
+__device__ __forceinline__ NtOperand ns_op(const uint16_t* base, int row0, int rows, int ld, int64_t plane) {
+  return {reinterpret_cast<const char*>(base + (int64_t)row0 * ld), (uint32_t)ld * 2u, rows - row0, plane * 2};
+}
+
+// upper-triangle tile t (row-major) of nt x nt tiles
+__device__ __forceinline__ void ns_tri(int t, int nt, int& ti, int& tj) {
+  ti = 0;
+  while (t >= nt - ti) {
+    t -= nt - ti;
+    ++ti;
+  }
+  tj = ti + t;
+}
+
+__device__ __forceinline__ void st4_pair(uint16_t* d, int64_t plane, const float v[4]) {
+  uint16_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split_f16(v[e], h[e], l[e]);
+  *reinterpret_cast<ushort4*>(d) = make_ushort4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(l[0], l[1], l[2], l[3]);
+}
+
+// Symmetric m x m products.  kGram: A = X X^T; kPoly: P = a I + b A + c A^2; kMul: L R of two slots.
+enum NsKind { kGram, kPoly, kMul };
+
+template <class C, int KIND>
+__global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int n_items, int ls, int rs, int ds) {
+  static_assert(C::BA == C::BB, "square tiles");
+  __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
+  int id = nt_xcd_item(blockIdx.x, n_items);
+  const int k = ns_find(p, id, &NsGroup::sym);
+  const NsGroup& g = p.g[k];
+  const int nt = (g.mp + C::BA - 1) / C::BA, tri = nt * (nt + 1) / 2;
+  const int mi = id / tri;
+  int ti, tj;
+  ns_tri(id % tri, nt, ti, tj);
+  const int64_t sp = (int64_t)g.mp * g.mp;
+  nt_f32x4 acc[C::TA][C::TB];
+  const int a0 = tj * C::BA, b0 = ti * C::BB;  // 4 consecutive elements of a lane run along rows of A: columns of C
+  if constexpr (KIND == kGram) {
+    const uint16_t* x = ns_x(p, g, mi);
+    const int64_t xp = (int64_t)g.mp * g.np;
+    nt_loop<C>(ring, ns_op(x, a0, g.mp, g.np, xp), ns_op(x, b0, g.mp, g.np, xp), 0, g.np * 2, acc);
+  } else {
+    const uint16_t *l = ns_sq(p, g, mi, ls), *r = ns_sq(p, g, mi, rs);
+    nt_loop<C>(ring, ns_op(l, a0, g.mp, g.mp, sp), ns_op(r, b0, g.mp, g.mp, sp), 0, g.mp * 2, acc);
+  }
+  uint16_t* dst = ns_sq(p, g, mi, ds);
+  const uint16_t* av = ns_sq(p, g, mi, kA);
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int wa = wid / C::WB, wb = wid % C::WB;
+  const float f = KIND == kGram ? 1.f / kNsX : KIND == kPoly ? 1.f / (kNsX * kNsX) : 1.f / kNsP;
+#pragma unroll
+  for (int i = 0; i < C::TA; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TB; ++j) {
+      const int ca = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;  // column of C
+      const int cb = b0 + (wb * C::TB + j) * 16 + (lane & 15);      // row of C
+      if (ca >= g.mp || cb >= g.mp) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
+      if constexpr (KIND == kPoly) {
+        const uint16_t* q = av + (int64_t)cb * g.mp + ca;
+        const ushort4 h = *reinterpret_cast<const ushort4*>(q), l = *reinterpret_cast<const ushort4*>(q + sp);
+        const float ah[4] = {f16_to_f32(h.x) + f16_to_f32(l.x), f16_to_f32(h.y) + f16_to_f32(l.y),
+                             f16_to_f32(h.z) + f16_to_f32(l.z), f16_to_f32(h.w) + f16_to_f32(l.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = kNsP * ((ca + e == cb ? kNsA : 0.f) + kNsB * (ah[e] / kNsX) + kNsC * v[e]);
+      }
+      if (ti != tj) st4_pair(dst + (int64_t)cb * g.mp + ca, sp, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (ca + e < cb && ti == tj) continue;  // the lower half of a diagonal tile comes from the upper
+        uint16_t h, l;
+        split_f16(v[e], h, l);
+        uint16_t* d = dst + (int64_t)(ca + e) * g.mp + cb;
+        d[0] = h;
+        d[sp] = l;
+        if (ti == tj) {
+          d = dst + (int64_t)cb * g.mp + ca + e;
+          d[0] = h;
+          d[sp] = l;
+        }
+      }
+    }
+}
+
+// X' = Q X.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X'
+// and its transpose (the other version) are stored for the next group of steps.
+template <class C, bool FINAL>
+__global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int n_items, int qs, int ver) {
+  __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
+  int id = nt_xcd_item(blockIdx.x, n_items);
+  const int k = ns_find(p, id, &NsGroup::rect);
+  const NsGroup& g = p.g[k];
+  const int mt = (g.mp + C::BA - 1) / C::BA, nt = (g.np + C::BA - 1) / C::BA;
+  const int mi = id / (mt * nt), t = id % (mt * nt);
+  const int m0 = t % mt * C::BA, n0 = t / mt * C::BA;
+  const int64_t sp = (int64_t)g.mp * g.mp, xp = (int64_t)g.mp * g.np;
+  // the operand whose rows are consecutive in the result's memory comes first (4 elements per lane)
+  const bool turned = FINAL && g.tall;
+  const NtOperand q = ns_op(ns_sq(p, g, mi, qs), m0, g.mp, g.mp, sp);
+  const NtOperand x = ns_op(ns_xt(p, g, mi, ver), n0, g.np, g.mp, xp);
+  NtOperand A = turned ? q : x, B = turned ? x : q;
+  nt_f32x4 acc[C::TA][C::TB];
+  nt_loop<C>(ring, A, B, 0, g.mp * 2, acc);
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int wa = wid / C::WB, wb = wid % C::WB;
+  const int a0 = turned ? m0 : n0, b0 = turned ? n0 : m0;
+  if constexpr (FINAL) {
+    const float f = 1.f / (kNsP * kNsX);
+    const int64_t off = p.off[g.first + mi];
+    const float lr = u.lr != nullptr ? *u.lr : 0.f;
+#pragma unroll
+    for (int i = 0; i < C::TA; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TB; ++j) {
+        const int c = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;
+        const int r = b0 + (wb * C::TB + j) * 16 + (lane & 15);
+        if (r >= g.rows || c >= g.cols) continue;
+        const int cnt = min(4, g.cols - c);
+        const int64_t at = off + (int64_t)r * g.cols + c;
+        const bool vec = u.vec && at % 4 == 0 && cnt == 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
+        if (u.w != nullptr) {
+          float w[4];
+          ns_ld4(u.w, at, 0, vec, cnt, w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = w[e] - lr * (g.scale * v[e] + u.wd * w[e]);
+        }
+        if (vec) {
+          st4c(u.out, at, u.out_code, 0, v);
+          if (u.shadow != nullptr) st4c(u.shadow, at, u.shadow_code, u.shadow_plane, v);
+        } else {
+          for (int e = 0; e < cnt; ++e) {
+            st(u.out, at + e, v[e], u.out_code);
+            if (u.shadow != nullptr) stc(u.shadow, at + e, v[e], u.shadow_code, u.shadow_plane);
+          }
+        }
+      }
+  } else {
+    uint16_t *dx = ns_x(p, g, mi), *dt = ns_xt(p, g, mi, ver ^ 1);
+#pragma unroll
+    for (int i = 0; i < C::TA; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TB; ++j) {
+        const int c = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;  // n
+        const int r = b0 + (wb * C::TB + j) * 16 + (lane & 15);      // m
+        if (r >= g.mp || c >= g.np) continue;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (1.f / kNsP);
+        st4_pair(dx + (int64_t)r * g.np + c, xp, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint16_t h, l;
+          split_f16(v[e], h, l);
+          uint16_t* d = dt + (int64_t)(c + e) * g.mp + r;
+          d[0] = h;
+          d[xp] = l;
+        }
+      }
+  }
+}
+
+using Tile64 = NtCfg<2, 64, 64, 2, 2, 4>;
+
+template <class C>
+void ns_chain(const NsArgs& p, const NsUpdate& u, int steps, int n_sym, int n_rect, hipStream_t st) {
+  int ver = 0;
+  for (int done = 0; done < steps;) {
+    int q = kP0;
+    ns_sym_kernel<C, kGram><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, 0, 0, kA);
+    ns_sym_kernel<C, kPoly><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kA, kA, kP0);
+    if (steps - done >= 2) {
+      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kP0, kA, kT);
+      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kT, kP0, kA);
+      ns_sym_kernel<C, kPoly><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kA, kA, kP1);
+      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kP1, kP0, kQ);
+      q = kQ;
+    }
+    done += q == kQ ? 2 : 1;
+    if (done < steps) ns_apply_kernel<C, false><<<n_rect, C::THREADS, 0, st>>>(p, u, n_rect, q, ver);
+    else ns_apply_kernel<C, true><<<n_rect, C::THREADS, 0, st>>>(p, u, n_rect, q, ver);
+    ver ^= 1;
+  }
+}
+
+}  // namespace
+
+void ns_shape(NsGroup& g) {
+  g.tall = g.rows > g.cols;
+  g.m = std::min(g.rows, g.cols);
+  g.n = std::max(g.rows, g.cols);
+  g.mp = (g.m + 63) / 64 * 64;
+  g.np = (g.n + 63) / 64 * 64;
+  const int64_t n = (int64_t)g.rows * g.cols;
+  g.run = (n + kNsParts - 1) / kNsParts;
+  g.run = std::max<int64_t>(4096, (g.run + 1023) / 1024 * 1024);
+  g.parts = (int)((n + g.run - 1) / g.run);
+  g.scale = (float)std::sqrt(std::max(1.0, (double)g.rows / g.cols));
+}
+
+int64_t ns_ws_elements(const NsGroup& g) { return g.count * (6 * (int64_t)g.mp * g.np + 2 * kSlots * (int64_t)g.mp * g.mp); }
+
+void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const NsUpdate& u, int steps, uint16_t* ws,
+            double* part, hipStream_t st) {
+  using C = Tile64;
+  NsArgs p = {};
+  p.ng = ng;
+  p.ws = ws;
+  p.part = part;
+  std::copy(off, off + nmats, p.off);
+  int64_t at = 0;
+  int first = 0, ew = 0, init = 0, sym = 0, rect = 0;
+  for (int k = 0; k < ng; ++k) {
+    NsGroup& g = p.g[k] = groups[k];
+    const int mt = (g.mp + C::BA - 1) / C::BA, nt = (g.np + C::BA - 1) / C::BA;
+    g.first = first;
+    g.ws = at;
+    g.ew = ew;
+    g.init = init;
+    g.sym = sym;
+    g.rect = rect;
+    first += g.count;
+    at += ns_ws_elements(g);
+    ew += g.count * g.parts;
+    init += g.count * (g.mp / 64) * (g.np / 64);
+    sym += g.count * mt * (mt + 1) / 2;
+    rect += g.count * mt * nt;
+  }
+  ns_norm_kernel<<<ew, 256, 0, st>>>(p, u);
+  ns_init_kernel<<<init, 256, 0, st>>>(p, u);
+  ns_chain<C>(p, u, steps, sym, rect, st);
+}
+
+}  // namespace mxr

@@ -11,3 +11,5 @@ from .roi_pool import roi_pool, roi_pool_bn_relu  # noqa: F401
 from .losses import rpn_softmax_ce, softmax_ce, smooth_l1  # noqa: F401
 from .bn import frozen_bn_relu  # noqa: F401
 from .sgd import sgd_momentum_  # noqa: F401
+from .muon import muon_update_, orthogonalize  # noqa: F401
+from .int8 import int8_linear, int8_matmul, quantize_rows  # noqa: F401

@@ -1,0 +1,330 @@
+"""Newton-Schulz orthogonalisation and the Muon update (ops/muon.py) against 64-bit computations.
+
+Tolerance of an orthogonalisation, of the result's norm: twice the error that the plain recurrence has in
+IEEE fp32 on the same input (rounding differs, its size and what the iteration makes of it do not), plus
+16 * 2^-23 for the 22-bit operands, plus eps / 2 of the output type.  A weight moves by lr * scale times
+that, and three fp32 roundings.
+"""
+import math
+
+import pytest
+import torch
+
+from mx_rcnn_amd import ops
+from mx_rcnn_amd.ops.muon import newton_schulz_ref
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+U32 = 2.0 ** -24
+
+
+@pytest.fixture
+def dev(request):
+    if request.param == 'cuda':
+        return request.getfixturevalue('cuda')
+    return torch.device('cpu')
+
+
+on_both = pytest.mark.parametrize('dev', DEVICES, indirect=True)
+
+
+def _ns64(g, steps=5, eps=1e-7):
+    """By singular values: U p(p(.. s)) V^T in 64 bits, p(s) = a s + b s^3 + c s^5."""
+    g = g.detach().cpu().double()
+    u, s, v = torch.linalg.svd(g, full_matrices=False)
+    s = s / (g.square().sum((-2, -1)).sqrt() + eps).unsqueeze(-1)
+    for _ in range(steps):
+        s = 3.4445 * s - 4.7750 * s ** 3 + 2.0315 * s ** 5
+    return (u * s.unsqueeze(-2)) @ v.contiguous()
+
+
+def _norm(x):
+    return x.double().flatten(-2).norm(dim=-1)
+
+
+def _tol(g, want, steps=5, eps=1e-7, dtype=torch.float32):
+    e32 = _norm(newton_schulz_ref(g.detach().cpu().float(), steps, eps).double() - want)
+    out = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    # where eps outweighs |G|, X0 is small and held at an absolute step: elements times 2^15 in fp16 pairs, whose
+    # subnormals are 2^-24 apart, so an element is off by at most 2^-25 * 2^-15 = 2^-40 and X by sqrt(r c) of
+    # that.  It is stored at the start and after every second step, and each remaining step multiplies by at
+    # most 3.4445: in all at most 3.4445^steps * (1 + 1 / 11.86 + ..) < 1.1 * 3.4445^steps times as much.
+    floor = 1.1 * 3.4445 ** steps * math.sqrt(g.shape[-2] * g.shape[-1]) * 2.0 ** -40
+    return 2 * e32 + (16 * 2.0 ** -23 + out) * _norm(want) + floor
+
+
+def _check(out, g, steps=5, eps=1e-7):
+    g3 = g if g.dim() == 3 else g[None]
+    o3 = out if out.dim() == 3 else out[None]
+    want = _ns64(g3, steps, eps)
+    assert out.dtype == g.dtype and out.shape == g.shape
+    over = _norm(o3.cpu().double() - want) - _tol(g3, want, steps, eps, g.dtype)
+    assert float(over.max()) <= 0, (over, _norm(want))
+
+
+def _matrix(b, r, c, kind, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    g = torch.randn(b, r, c, generator=gen, dtype=torch.float64)
+    if kind != 'noise':
+        u, s, v = torch.linalg.svd(g, full_matrices=False)
+        k = s.shape[-1]
+        i = torch.arange(k).double()
+        s = {'power': 1 / (i + 1), 'steep': torch.exp(-12 * i / k), 'rank': (i < max(1, k // 8)).double(),
+             'peak': torch.where(i == 0, 1.0, 2e-3)}[kind].expand_as(s)
+        g = (u * s.unsqueeze(-2)) @ v.contiguous()
+    return (g * 1e-3).float()
+
+
+@on_both
+@pytest.mark.parametrize('b,r,c', [
+    (1, 1, 1), (1, 1, 100), (1, 100, 1), (2, 2, 3), (1, 16, 16), (3, 63, 65), (1, 64, 64), (1, 64, 576), (2, 65, 147),
+    (1, 130, 70), (2, 200, 64), (1, 128, 1000), (1, 257, 300), (1, 384, 130)])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_orthogonalize(dev, b, r, c, dtype):
+    g = _matrix(b, r, c, 'noise', seed=r + c).to(dtype)
+    _check(ops.orthogonalize(g.to(dev)), g)
+    _check(ops.orthogonalize(g[0].to(dev)), g[0])
+
+
+@on_both
+@pytest.mark.parametrize('kind', ['power', 'steep', 'rank', 'peak'])
+@pytest.mark.parametrize('r,c', [(64, 576), (256, 96), (192, 192)])
+def test_orthogonalize_spectra(dev, kind, r, c):
+    g = _matrix(2, r, c, kind)
+    _check(ops.orthogonalize(g.to(dev)), g)
+
+
+@on_both
+@pytest.mark.parametrize('steps', [1, 2, 3, 4, 6, 7])
+def test_orthogonalize_steps(dev, steps):
+    g = _matrix(2, 48, 200, 'power')
+    _check(ops.orthogonalize(g.to(dev), steps=steps), g, steps=steps)
+
+
+@on_both
+def test_orthogonalize_scales(dev):
+    """Tiny and huge gradients (the squares leave fp32), eps that counts, zeros."""
+    g = _matrix(6, 40, 90, 'noise')
+    g = g / _norm(g).float()[:, None, None]
+    g = g * torch.tensor([1.0, 1e-30, 1e30, 1e-7, 1e-12, 0.0])[:, None, None]
+    out = ops.orthogonalize(g.to(dev))
+    _check(out, g)
+    assert (out[5] == 0).all() and torch.isfinite(out[[0, 3, 4]]).all()
+    _check(ops.orthogonalize(g[:1].to(dev), eps=0.5), g[:1], eps=0.5)
+
+
+@on_both
+def test_orthogonalize_nonfinite_stays_in_its_matrix(dev):
+    g = _matrix(4, 30, 80, 'noise')
+    g[1, 3, 5] = float('nan')
+    g[2, 29, 79] = float('inf')
+    out = ops.orthogonalize(g.to(dev)).cpu()
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all()
+    _check(out[[0, 3]], g[[0, 3]])
+
+
+@on_both
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_orthogonalize_strided(dev, dtype):
+    base = _matrix(3, 70, 90, 'noise').to(dtype).to(dev)
+    for g in (base[:, ::2], base[:, 1:, 3:], base.transpose(1, 2), base[1:2, :, :50], base[0].t()):
+        _check(ops.orthogonalize(g), g)
+    for shape in ((0, 4, 4), (0, 5), (3, 0, 2)):
+        assert ops.orthogonalize(torch.empty(shape, dtype=dtype, device=dev)).shape == shape
+
+
+@pytest.mark.gpu
+def test_orthogonalize_many_equals_one_by_one(cuda):
+    """More matrices than one launch carries, each with the bits that it has alone."""
+    g = _matrix(131, 20, 45, 'noise').to(cuda)
+    out = ops.orthogonalize(g)
+    for k in (0, 1, 64, 127, 128, 130):
+        assert torch.equal(out[k], ops.orthogonalize(g[k]))
+    assert torch.equal(out, ops.orthogonalize(g))
+
+
+def _update64(w, mom, grad, mats, lr, mu, wd, rescale, clip, nesterov, steps):
+    w, mom, g = [t.detach().cpu().double().clone() for t in (w, mom, grad)]
+    g = g * rescale
+    if clip > 0:
+        g = g.clamp(-clip, clip)
+    tol = torch.zeros_like(w)
+    for o, r, c in mats:
+        s = slice(o, o + r * c)
+        mom[s] = mu * mom[s] + g[s]
+        u = (g[s] + mu * mom[s] if nesterov else mom[s]).view(1, r, c)
+        d = _ns64(u, steps)
+        k = math.sqrt(max(1.0, r / c))
+        # norm of the allowed difference, spread over the matrix (compared as a norm below)
+        tol[s] = lr * k * float(_tol(u, d, steps)[0]) / math.sqrt(r * c)
+        w[s] -= lr * (k * d.reshape(-1) + wd * w[s])
+    return w, mom, tol
+
+
+def _flat(n, dev, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [(torch.randn(n, generator=gen) * k).to(dev) for k in (0.02, 5e-3, 1e-3)]
+
+
+def _check_update(dev, mats, n, gdtype=torch.float32, mu=0.95, wd=5e-4, rescale=1.0, clip=-1.0, nesterov=True, steps=5,
+                  planes=0, zero=None, seed=0):
+    w, mom, grad = _flat(n, dev, seed)
+    grad = grad.to(gdtype)
+    lr = torch.full((1,), 0.02, device=dev)
+    w0, m0, g0 = w.clone(), mom.clone(), grad.clone()
+    shadow = torch.full((max(planes, 1) * ((n + 7) // 8 * 8),), 7.0, dtype=torch.bfloat16, device=dev) if planes else None
+    z = {'same': grad, 'other': torch.ones(n, dtype=torch.bfloat16, device=dev), None: None}[zero]
+    ops.muon_update_(w, mom, grad, mats, lr, momentum=mu, wd=wd, rescale=rescale, clip=clip, nesterov=nesterov,
+                     steps=steps, w_bf16=shadow, planes=max(planes, 1), zero=z)
+    want, mwant, tol = _update64(w0, m0, g0, mats, float(lr), mu, wd, rescale, clip, nesterov, steps)
+    inside = torch.zeros(n, dtype=torch.bool)
+    for o, r, c in mats:
+        s = slice(o, o + r * c)
+        inside[s] = True
+        d = (w[s].cpu().double() - want[s]).norm()
+        assert float(d) <= float(tol[s].norm()) + 3 * U32 * float(want[s].norm() + w0[s].cpu().double().norm())
+        md = (mom[s].cpu().double() - mwant[s]).abs()
+        mtol = 3 * U32 * (m0[s].cpu().double().abs() + (g0[s].cpu().double() * rescale).abs())
+        assert bool((md <= mtol).all())
+    out = ~inside
+    assert torch.equal(w.cpu()[out], w0.cpu()[out]) and torch.equal(mom.cpu()[out], m0.cpu()[out])
+    if z is not None:
+        assert (z.cpu()[inside] == 0).all()
+        keep = g0.cpu() if zero == 'same' else torch.ones(n, dtype=torch.bfloat16)
+        assert torch.equal(z.cpu()[out], keep[out])
+    if planes:
+        pl = shadow.numel() // planes
+        parts = [shadow[k * pl:k * pl + n].cpu() for k in range(planes)]
+        if planes == 1:
+            assert torch.equal(parts[0][inside], w.cpu().bfloat16()[inside])
+        elif planes == 3:
+            assert torch.equal((parts[0].float() + parts[1].float() + parts[2].float())[inside], w.cpu()[inside])
+        else:
+            err = ((parts[0].float() + parts[1].float()) - w.cpu()).abs()
+            assert bool((err <= 2.0 ** -16 * w.cpu().abs())[inside].all())
+        for p in parts:
+            assert (p[out].float() == 7).all()
+    return w, mom
+
+
+MATS = ((0, 64, 147), (9408 + 5, 64, 64), (13600, 100, 30), (16700, 30, 100), (20000, 1, 64), (20070, 64, 1))
+SIZE = 20141
+
+
+@on_both
+@pytest.mark.parametrize('gdtype', DTYPES)
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_muon_update(dev, gdtype, nesterov):
+    _check_update(dev, MATS, SIZE, gdtype, nesterov=nesterov)
+
+
+@on_both
+@pytest.mark.parametrize('planes', [1, 2, 3])
+@pytest.mark.parametrize('zero', [None, 'same', 'other'])
+def test_muon_update_shadow_and_clear(dev, planes, zero):
+    _check_update(dev, MATS, SIZE, planes=planes, zero=zero)
+
+
+@on_both
+@pytest.mark.parametrize('kw', [{'rescale': 0.25}, {'clip': 1e-3}, {'rescale': 3.0, 'clip': 2e-3}, {'mu': 0.0}, {'wd': 0.0},
+                                {'steps': 3}])
+def test_muon_update_options(dev, kw):
+    _check_update(dev, MATS, SIZE, **kw)
+
+
+@on_both
+def test_muon_update_no_matrices(dev):
+    w, mom, grad = _flat(100, dev)
+    before = w.clone()
+    ops.muon_update_(w, mom, grad, (), torch.ones(1, device=dev))
+    assert torch.equal(w, before)
+
+
+@pytest.mark.gpu
+def test_muon_update_many_shapes(cuda):
+    """More shapes than one launch carries, in any order, at any offset."""
+    mats, at = [], 3
+    for k in range(40):
+        r, c = 5 + 3 * (k % 20), 90 - 4 * (k % 20)
+        mats.append((at, r, c))
+        at += r * c + k % 3
+    mats = tuple(mats[::-1])
+    w, mom = _check_update(cuda, mats, at + 10)
+    w2, mom2 = _check_update(cuda, mats, at + 10)
+    assert torch.equal(w, w2) and torch.equal(mom, mom2)
+
+
+@on_both
+def test_muon_refusals(dev):
+    w, mom, grad = _flat(1000, dev)
+    lr = torch.ones(1, device=dev)
+    bad = [dict(mats=((0, 10, 101),)), dict(mats=((-1, 10, 10),)), dict(mats=((0, 10, 10), (99, 5, 5))),
+           dict(mats=((0, 0, 10),)), dict(mats=((0, 10, 10),), steps=0), dict(mats=((0, 10, 10),), steps=17),
+           dict(mats=((0, 10, 10),), eps=0.0), dict(mats=((0, 17000, 17000),))]
+    before = [t.clone() for t in (w, mom, grad)]
+    for kw in bad:
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.muon_update_(w, mom, grad, kw.pop('mats'), lr, **kw)
+    for g in (torch.ones(4, device=dev), torch.ones(2, 3, 4, 5, device=dev), torch.ones(3, 3, device=dev).double(),
+              torch.ones(3, 3, device=dev, dtype=torch.int32)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            ops.orthogonalize(g)
+    for kw in ({'steps': 0}, {'steps': 2.5}, {'eps': -1.0}):
+        with pytest.raises(ValueError):
+            ops.orthogonalize(torch.ones(3, 3, device=dev), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(before, (w, mom, grad)))
+
+
+@pytest.mark.gpu
+def test_muon_refuses_wrong_tensors(cuda):
+    w, mom, grad = _flat(400, cuda)
+    lr = torch.ones(1, device=cuda)
+    mats = ((0, 10, 10),)
+    for c in ((w.half(), mom, grad, mats, lr), (w, mom[:300], grad, mats, lr), (w, mom, grad.cpu(), mats, lr),
+              (w, mom.cpu(), grad, mats, lr), (w, mom, grad, mats, lr.cpu()), (w, mom, grad.double(), mats, lr),
+              (w, mom, grad, mats, lr.expand(2).contiguous())):
+        with pytest.raises(RuntimeError):
+            ops.muon_update_(*c)
+    with pytest.raises(RuntimeError):
+        ops.muon_update_(w, mom, grad, mats, lr, w_bf16=torch.empty(300, dtype=torch.bfloat16, device=cuda))
+    with pytest.raises(RuntimeError):
+        ops.muon_update_(w, mom, grad, mats, lr, zero=grad[:300])
+
+
+@pytest.mark.gpu
+def test_muon_graph_and_streams(cuda):
+    """Two captured updates of the same shapes, replayed in turn with eager ones between: the weights of
+    eager updates, bit for bit."""
+    states = [_flat(SIZE, cuda, seed=k) for k in range(3)]
+    lr = torch.full((1,), 0.02, device=cuda)
+    grads = [_flat(SIZE, cuda, seed=10 + k)[2] for k in range(4)]
+
+    def update(st, g):
+        ops.muon_update_(st[0], st[1], g, MATS, lr, wd=5e-4)
+
+    eager = [[t.clone() for t in st] for st in states]
+    for g in grads:
+        for st in eager:
+            update(st, g)
+    static = grads[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = [t.clone() for t in states[0]]
+        update(warm, static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for st in states[:2]:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            update(st, static)
+        graphs.append(gr)
+    for g in grads:
+        static.copy_(g)
+        graphs[0].replay()
+        update(states[2], g)
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    for st, want in zip(states, eager):
+        assert torch.equal(st[0], want[0]) and torch.equal(st[1], want[1])
