@@ -97,18 +97,18 @@ __global__ void __launch_bounds__(C::THREADS) int8_tile_kernel(Int8Args p, int n
   const int sp = id / (nt * mt), t = id % (nt * mt);
   const int n0 = t / mt * C::BA;
   const int64_t m0 = (int64_t)(t % mt) * C::BB;
-  const NtOperand A = {reinterpret_cast<const char*>(p.w) + n0 * p.ldw, (uint32_t)p.ldw, p.N - n0, 0};
-  const NtOperand B = {reinterpret_cast<const char*>(p.x) + m0 * p.ldx, (uint32_t)p.ldx,
-                       (int)min((int64_t)C::BB, p.M - m0), 0};
+  const NtOperand A = {reinterpret_cast<const char*>(p.w) + n0 * p.ldw, p.N - n0, (uint32_t)p.ldw, 0};
+  const NtOperand B = {reinterpret_cast<const char*>(p.x) + m0 * p.ldx, (int)min((int64_t)C::BB, p.M - m0),
+                       (uint32_t)p.ldx, 0};
   typename C::Acc acc[C::TA][C::TB];
   const int k0 = sp * run;
   nt_loop<C>(ring, A, B, k0, min(p.K, k0 + run), acc);
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wa = wid / C::WB, wb = wid % C::WB;
+  const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
 #pragma unroll
   for (int i = 0; i < C::TA; ++i)
 #pragma unroll
     for (int j = 0; j < C::TB; ++j) {
+      if (!C::mine(i, j)) continue;
       const int n = n0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;
       const int64_t m = m0 + (wb * C::TB + j) * 16 + (lane & 15);
       if (m >= p.M || n >= p.N) continue;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) int8_join_kernel(Int8Args p, int splits, 
   }
 }
 
-using Int8Tile = NtCfg<1, 64, 64, 2, 2, 4>;
+using Int8Tile = NtCfg<false, 64, 64, 1, 2, 2, 4>;
 
 struct Int8Plan {
   bool pack;
@@ -164,10 +164,10 @@ Int8Plan int8_plan(const Int8Args& a) {
   p.lda = (a.K + 15) / 16 * 16;
   p.nt = div_up(a.N, C::BA);
   p.mt = div_up(a.M, C::BB);
-  const int nk = div_up(p.lda, 64);
+  const int nk = div_up(p.lda, 128);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ((int64_t)p.nt * p.mt), nk / 8));
-  p.run = std::max(1, div_up(nk, p.splits)) * 64;
-  p.splits = std::max(1, div_up(nk * 64, p.run));
+  p.run = std::max(1, div_up(nk, p.splits)) * 128;
+  p.splits = std::max(1, div_up(nk * 128, p.run));
   p.pack_bytes = p.pack ? ((a.M + a.N) * p.lda + 255) / 256 * 256 : 0;
   p.bytes = p.pack_bytes + (p.splits > 1 ? p.splits * a.M * a.N * 4 : 0);
   return p;

@@ -52,23 +52,36 @@ __device__ __forceinline__ int ns_find(const NsArgs& p, int& id, int NsGroup::*s
   return k;
 }
 
-__device__ __forceinline__ int64_t ns_stride(const NsGroup& g) {
-  return 6 * (int64_t)g.mp * g.np + 2 * kSlots * (int64_t)g.mp * g.mp;
+// Buffers hold fp16 pairs in panels (tile_nt.h): for every 32 columns, the lines of all rows, each 32 hi and 32 lo.
+__host__ __device__ __forceinline__ int64_t ns_size(int rows, int cols) { return (int64_t)rows * cols * 2; }
+__host__ __device__ __forceinline__ int64_t ns_stride(const NsGroup& g) {  // of one matrix, in fp16 elements
+  return 3 * ns_size(g.mp, g.np) + kSlots * ns_size(g.mp, g.mp);
 }
-// planes of matrix mi of group g: X (mp x np), its transpose in two versions (np x mp), m x m slots
+// matrix mi of group g: X (mp x np), its transpose in two versions (np x mp), m x m slots
 __device__ __forceinline__ uint16_t* ns_x(const NsArgs& p, const NsGroup& g, int mi) {
   return p.ws + g.ws + mi * ns_stride(g);
 }
 __device__ __forceinline__ uint16_t* ns_xt(const NsArgs& p, const NsGroup& g, int mi, int ver) {
-  return ns_x(p, g, mi) + (2 + 2 * ver) * (int64_t)g.mp * g.np;
+  return ns_x(p, g, mi) + (1 + ver) * ns_size(g.mp, g.np);
 }
 __device__ __forceinline__ uint16_t* ns_sq(const NsArgs& p, const NsGroup& g, int mi, int slot) {
-  return ns_x(p, g, mi) + 6 * (int64_t)g.mp * g.np + slot * 2 * (int64_t)g.mp * g.mp;
+  return ns_x(p, g, mi) + 3 * ns_size(g.mp, g.np) + slot * ns_size(g.mp, g.mp);
 }
 
 __device__ __forceinline__ void split_f16(float v, uint16_t& hi, uint16_t& lo) {
   hi = f32_to_f16(v);
   lo = f32_to_f16(v - f16_to_f32(hi));
+}
+// element (row, col) of a pair buffer of `rows` rows: its hi value; the lo value is 32 further
+__device__ __forceinline__ int64_t ns_at(int row, int rows, int col) {
+  return ((int64_t)(col >> 5) * rows + row) * 64 + (col & 31);
+}
+__device__ __forceinline__ void st4_pair(uint16_t* d, const float v[4]) {  // 4 columns, the first a multiple of 4
+  uint16_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split_f16(v[e], h[e], l[e]);
+  *reinterpret_cast<ushort4*>(d) = make_ushort4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<ushort4*>(d + 32) = make_ushort4(l[0], l[1], l[2], l[3]);
 }
 
 // ---- the values that are orthogonalised ---------------------------------------------------------
@@ -179,31 +192,38 @@ __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
     for (int e = 0; e < 4; ++e) tile[lr + 16 * q][lc + e] = v[e];
   }
   __syncthreads();
-  const int64_t plane = (int64_t)g.mp * g.np;
   uint16_t* same = g.tall ? ns_xt(p, g, mi, 0) : ns_x(p, g, mi);   // laid out as in memory
   uint16_t* turn = g.tall ? ns_x(p, g, mi) : ns_xt(p, g, mi, 0);
-  const int lds_ = g.tall ? g.mp : g.np, ldt = g.tall ? g.np : g.mp;
+  const int rs = g.tall ? g.np : g.mp, rq = g.tall ? g.mp : g.np;  // their rows
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int a = lr + 16 * q;
-    uint16_t h[4], l[4], ht[4], lt[4];
+    float v[4], t[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      split_f16(tile[a][lc + e], h[e], l[e]);
-      split_f16(tile[lc + e][a], ht[e], lt[e]);
+      v[e] = tile[a][lc + e];
+      t[e] = tile[lc + e][a];
     }
-    uint16_t* d = same + (int64_t)(r0 + a) * lds_ + c0 + lc;
-    *reinterpret_cast<ushort4*>(d) = make_ushort4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(l[0], l[1], l[2], l[3]);
-    d = turn + (int64_t)(c0 + a) * ldt + r0 + lc;
-    *reinterpret_cast<ushort4*>(d) = make_ushort4(ht[0], ht[1], ht[2], ht[3]);
-    *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(lt[0], lt[1], lt[2], lt[3]);
+    st4_pair(same + ns_at(r0 + a, rs, c0 + lc), v);
+    st4_pair(turn + ns_at(c0 + a, rq, r0 + lc), t);
   }
 }
 
 // ---- products -----------------------------------------------------------------------------------
-__device__ __forceinline__ NtOperand ns_op(const uint16_t* base, int row0, int rows, int ld, int64_t plane) {
-  return {reinterpret_cast<const char*>(base + (int64_t)row0 * ld), (uint32_t)ld * 2u, rows - row0, plane * 2};
+__device__ __forceinline__ NtOperand ns_op(const uint16_t* base, int row0, int rows) {
+  return {reinterpret_cast<const char*>(base + (int64_t)row0 * 64), rows - row0, 0, (int64_t)rows * 128};
+}
+
+// A 16 x 16 tile turned within the wave: lane l holds rows 4 (l >> 4) .. + 3 of column l & 15, and gets columns
+// 4 (l >> 4) .. + 3 of row l & 15.  `s`: 16 x 20 floats of this wave alone (its LDS accesses stay in order).
+__device__ __forceinline__ void ns_turn(float* s, int lane, const float v[4], float t[4]) {
+  const int g = lane >> 4, r = lane & 15;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[(4 * g + e) * 20 + r] = v[e];
+  __builtin_amdgcn_wave_barrier();
+  const float4 q = *reinterpret_cast<const float4*>(s + r * 20 + 4 * g);
+  __builtin_amdgcn_wave_barrier();
+  t[0] = q.x; t[1] = q.y; t[2] = q.z; t[3] = q.w;
 }
 
 // upper-triangle tile t (row-major) of nt x nt tiles
@@ -216,77 +236,72 @@ __device__ __forceinline__ void ns_tri(int t, int nt, int& ti, int& tj) {
   tj = ti + t;
 }
 
-__device__ __forceinline__ void st4_pair(uint16_t* d, int64_t plane, const float v[4]) {
-  uint16_t h[4], l[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) split_f16(v[e], h[e], l[e]);
-  *reinterpret_cast<ushort4*>(d) = make_ushort4(h[0], h[1], h[2], h[3]);
-  *reinterpret_cast<ushort4*>(d + plane) = make_ushort4(l[0], l[1], l[2], l[3]);
-}
-
 // Symmetric m x m products.  kGram: A = X X^T; kPoly: P = a I + b A + c A^2; kMul: L R of two slots.
 enum NsKind { kGram, kPoly, kMul };
 
 template <class C, int KIND>
-__global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int n_items, int ls, int rs, int ds) {
+__global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int ls, int rs, int ds) {
   static_assert(C::BA == C::BB, "square tiles");
   __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
-  int id = nt_xcd_item(blockIdx.x, n_items);
-  const int k = ns_find(p, id, &NsGroup::sym);
+  int id = blockIdx.x;
+  const int k = ns_find(p, id, KIND == kGram ? &NsGroup::gram : &NsGroup::sym);
   const NsGroup& g = p.g[k];
   const int nt = (g.mp + C::BA - 1) / C::BA, tri = nt * (nt + 1) / 2;
+  id = nt_xcd_item(id, g.count * tri);
   const int mi = id / tri;
   int ti, tj;
   ns_tri(id % tri, nt, ti, tj);
-  const int64_t sp = (int64_t)g.mp * g.mp;
   nt_f32x4 acc[C::TA][C::TB];
   const int a0 = tj * C::BA, b0 = ti * C::BB;  // 4 consecutive elements of a lane run along rows of A: columns of C
   if constexpr (KIND == kGram) {
     const uint16_t* x = ns_x(p, g, mi);
-    const int64_t xp = (int64_t)g.mp * g.np;
-    nt_loop<C>(ring, ns_op(x, a0, g.mp, g.np, xp), ns_op(x, b0, g.mp, g.np, xp), 0, g.np * 2, acc);
+    nt_loop<C>(ring, ns_op(x, a0, g.mp), ns_op(x, b0, g.mp), 0, g.np * 4, acc);
   } else {
     const uint16_t *l = ns_sq(p, g, mi, ls), *r = ns_sq(p, g, mi, rs);
-    nt_loop<C>(ring, ns_op(l, a0, g.mp, g.mp, sp), ns_op(r, b0, g.mp, g.mp, sp), 0, g.mp * 2, acc);
+    nt_loop<C>(ring, ns_op(l, a0, g.mp), ns_op(r, b0, g.mp), 0, g.mp * 4, acc);
   }
+  float* scratch = C::scratch(ring);
   uint16_t* dst = ns_sq(p, g, mi, ds);
   const uint16_t* av = ns_sq(p, g, mi, kA);
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wa = wid / C::WB, wb = wid % C::WB;
+  const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
   const float f = KIND == kGram ? 1.f / kNsX : KIND == kPoly ? 1.f / (kNsX * kNsX) : 1.f / kNsP;
 #pragma unroll
   for (int i = 0; i < C::TA; ++i)
 #pragma unroll
     for (int j = 0; j < C::TB; ++j) {
+      if (!C::mine(i, j)) continue;
       const int ca = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;  // column of C
       const int cb = b0 + (wb * C::TB + j) * 16 + (lane & 15);      // row of C
-      if (ca >= g.mp || cb >= g.mp) continue;
+      if (a0 + (wa * C::TA + i) * 16 >= g.mp || b0 + (wb * C::TB + j) * 16 >= g.mp) continue;  // (wave-uniform)
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
       if constexpr (KIND == kPoly) {
-        const uint16_t* q = av + (int64_t)cb * g.mp + ca;
-        const ushort4 h = *reinterpret_cast<const ushort4*>(q), l = *reinterpret_cast<const ushort4*>(q + sp);
+        const uint16_t* q = av + ns_at(cb, g.mp, ca);
+        const ushort4 h = *reinterpret_cast<const ushort4*>(q), l = *reinterpret_cast<const ushort4*>(q + 32);
         const float ah[4] = {f16_to_f32(h.x) + f16_to_f32(l.x), f16_to_f32(h.y) + f16_to_f32(l.y),
                              f16_to_f32(h.z) + f16_to_f32(l.z), f16_to_f32(h.w) + f16_to_f32(l.w)};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           v[e] = kNsP * ((ca + e == cb ? kNsA : 0.f) + kNsB * (ah[e] / kNsX) + kNsC * v[e]);
       }
-      if (ti != tj) st4_pair(dst + (int64_t)cb * g.mp + ca, sp, v);
+      // the turned tile: rows ca.., columns cb..; the lower half of a diagonal block comes from the upper half
+      float t[4];
+      ns_turn(scratch, lane, v, t);
+      const int ra = a0 + (wa * C::TA + i) * 16 + (lane & 15), rb = b0 + (wb * C::TB + j) * 16 + (lane >> 4) * 4;
+      if (ti != tj) {
+        st4_pair(dst + ns_at(cb, g.mp, ca), v);
+        st4_pair(dst + ns_at(ra, g.mp, rb), t);
+        continue;
+      }
+      const int tile_a = wa * C::TA + i, tile_b = wb * C::TB + j;
+      if (tile_a > tile_b) {
+        st4_pair(dst + ns_at(cb, g.mp, ca), v);
+        st4_pair(dst + ns_at(ra, g.mp, rb), t);
+      } else if (tile_a == tile_b) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (ca + e < cb && ti == tj) continue;  // the lower half of a diagonal tile comes from the upper
-        uint16_t h, l;
-        split_f16(v[e], h, l);
-        uint16_t* d = dst + (int64_t)(ca + e) * g.mp + cb;
-        d[0] = h;
-        d[sp] = l;
-        if (ti == tj) {
-          d = dst + (int64_t)cb * g.mp + ca + e;
-          d[0] = h;
-          d[sp] = l;
-        }
+        for (int e = 0; e < 4; ++e) v[e] = ca + e >= cb ? v[e] : t[e];
+        st4_pair(dst + ns_at(cb, g.mp, ca), v);
       }
     }
 }
@@ -294,24 +309,23 @@ __global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int n_item
 // X' = Q X.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X'
 // and its transpose (the other version) are stored for the next group of steps.
 template <class C, bool FINAL>
-__global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int n_items, int qs, int ver) {
+__global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int qs, int ver) {
   __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
-  int id = nt_xcd_item(blockIdx.x, n_items);
+  int id = blockIdx.x;
   const int k = ns_find(p, id, &NsGroup::rect);
   const NsGroup& g = p.g[k];
   const int mt = (g.mp + C::BA - 1) / C::BA, nt = (g.np + C::BA - 1) / C::BA;
+  id = nt_xcd_item(id, g.count * mt * nt);
   const int mi = id / (mt * nt), t = id % (mt * nt);
   const int m0 = t % mt * C::BA, n0 = t / mt * C::BA;
-  const int64_t sp = (int64_t)g.mp * g.mp, xp = (int64_t)g.mp * g.np;
   // the operand whose rows are consecutive in the result's memory comes first (4 elements per lane)
   const bool turned = FINAL && g.tall;
-  const NtOperand q = ns_op(ns_sq(p, g, mi, qs), m0, g.mp, g.mp, sp);
-  const NtOperand x = ns_op(ns_xt(p, g, mi, ver), n0, g.np, g.mp, xp);
+  const NtOperand q = ns_op(ns_sq(p, g, mi, qs), m0, g.mp);
+  const NtOperand x = ns_op(ns_xt(p, g, mi, ver), n0, g.np);
   NtOperand A = turned ? q : x, B = turned ? x : q;
   nt_f32x4 acc[C::TA][C::TB];
-  nt_loop<C>(ring, A, B, 0, g.mp * 2, acc);
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wa = wid / C::WB, wb = wid % C::WB;
+  nt_loop<C>(ring, A, B, 0, g.mp * 4, acc);
+  const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
   const int a0 = turned ? m0 : n0, b0 = turned ? n0 : m0;
   if constexpr (FINAL) {
     const float f = 1.f / (kNsP * kNsX);
@@ -321,6 +335,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
     for (int i = 0; i < C::TA; ++i)
 #pragma unroll
       for (int j = 0; j < C::TB; ++j) {
+        if (!C::mine(i, j)) continue;
         const int c = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;
         const int r = b0 + (wb * C::TB + j) * 16 + (lane & 15);
         if (r >= g.rows || c >= g.cols) continue;
@@ -347,51 +362,97 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
         }
       }
   } else {
+    float* scratch = C::scratch(ring);
     uint16_t *dx = ns_x(p, g, mi), *dt = ns_xt(p, g, mi, ver ^ 1);
 #pragma unroll
     for (int i = 0; i < C::TA; ++i)
 #pragma unroll
       for (int j = 0; j < C::TB; ++j) {
-        const int c = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;  // n
-        const int r = b0 + (wb * C::TB + j) * 16 + (lane & 15);      // m
-        if (r >= g.mp || c >= g.np) continue;
-        float v[4];
+        if (!C::mine(i, j)) continue;
+        if (b0 + (wb * C::TB + j) * 16 >= g.mp || a0 + (wa * C::TA + i) * 16 >= g.np) continue;  // (wave-uniform)
+        const int ca = a0 + (wa * C::TA + i) * 16, cb = b0 + (wb * C::TB + j) * 16;  // first n, first m of the tile
+        float v[4], t[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (1.f / kNsP);
-        st4_pair(dx + (int64_t)r * g.np + c, xp, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint16_t h, l;
-          split_f16(v[e], h, l);
-          uint16_t* d = dt + (int64_t)(c + e) * g.mp + r;
-          d[0] = h;
-          d[xp] = l;
-        }
+        ns_turn(scratch, lane, v, t);
+        st4_pair(dx + ns_at(cb + (lane & 15), g.mp, ca + (lane >> 4) * 4), v);
+        st4_pair(dt + ns_at(ca + (lane & 15), g.np, cb + (lane >> 4) * 4), t);
       }
   }
 }
 
-using Tile64 = NtCfg<2, 64, 64, 2, 2, 4>;
+// Tiles and their measured cost: microseconds per K tile with one block per CU alone and with every slot taken, slots
+// (blocks resident on the chip), and microseconds of start and epilogue per round.  Larger tiles read fewer bytes
+// per product, smaller ones fill the chip: 4096 x 4096 (us for a symmetric product / for P X) 64: 330 / 640, 128:
+// 262 / 380, 192: 222 / 410 (253 tiles, one round), 256: 265 (136 tiles on 256 CUs) / 313; ResNet-101's 84
+// matrices 64: 40 / 316, 128: 42 / 211, 192: 65 / 254, 256: 91 / 202.
+using Tile64 = NtCfg<true, 64, 64, 2, 2, 2, 2, 4, true>;  // two K groups: short products are bound by latency
+using Tile128 = NtCfg<true, 128, 128, 1, 2, 4, 2, 8>;
+using Tile192 = NtCfg<true, 192, 192, 1, 2, 4, 3, 8>;
+using Tile256 = NtCfg<true, 256, 256, 1, 2, 4, 2>;  // (no registers for sums in runs)
 
-template <class C>
-void ns_chain(const NsArgs& p, const NsUpdate& u, int steps, int n_sym, int n_rect, hipStream_t st) {
-  int ver = 0;
-  for (int done = 0; done < steps;) {
-    int q = kP0;
-    ns_sym_kernel<C, kGram><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, 0, 0, kA);
-    ns_sym_kernel<C, kPoly><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kA, kA, kP0);
-    if (steps - done >= 2) {
-      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kP0, kA, kT);
-      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kT, kP0, kA);
-      ns_sym_kernel<C, kPoly><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kA, kA, kP1);
-      ns_sym_kernel<C, kMul><<<n_sym, C::THREADS, 0, st>>>(p, n_sym, kP1, kP0, kQ);
-      q = kQ;
+struct NsTile {
+  int size, slots;
+  double alone, full, round;
+};
+constexpr NsTile kNsTiles[4] = {
+    {64, 512, 0.33, 0.64, 5.0}, {128, 512, 0.75, 1.40, 7.0}, {192, 256, 1.31, 1.68, 9.0}, {256, 256, 1.95, 2.45, 12.0}};
+
+enum NsLaunch { kLaunchGram, kLaunchSym, kLaunchRect };
+
+int ns_tiles(const NsGroup& g, int size, NsLaunch what) {
+  const int mt = (g.mp + size - 1) / size, nt = (g.np + size - 1) / size;
+  return g.count * (what == kLaunchRect ? mt * nt : mt * (mt + 1) / 2);
+}
+
+// The tile for one kind of launch: the groups' tiles dealt out in rounds, longest K first.
+int ns_pick(const NsGroup* g, int ng, NsLaunch what) {
+  int best = 0;
+  double least = 1e30;
+  for (int t = 0; t < 4; ++t) {
+    const NsTile& c = kNsTiles[t];
+    double us = 0;
+    int filled = 0, k_round = 0;
+    for (int i = 0; i < ng; ++i) {
+      const int k = (what == kLaunchGram ? g[i].np : g[i].mp) / 32;
+      for (int n = ns_tiles(g[i], c.size, what); n > 0;) {
+        if (filled == 0) k_round = 0;
+        k_round = std::max(k_round, k);
+        const int take = std::min(n, c.slots - filled);
+        n -= take;
+        filled += take;
+        if (filled == c.slots) {
+          us += k_round * c.full + c.round;
+          filled = 0;
+          // whole rounds of this group alone
+          us += (n / c.slots) * (k * c.full + c.round);
+          n %= c.slots;
+        }
+      }
     }
-    done += q == kQ ? 2 : 1;
-    if (done < steps) ns_apply_kernel<C, false><<<n_rect, C::THREADS, 0, st>>>(p, u, n_rect, q, ver);
-    else ns_apply_kernel<C, true><<<n_rect, C::THREADS, 0, st>>>(p, u, n_rect, q, ver);
-    ver ^= 1;
+    if (filled > 0) us += k_round * (c.alone + (c.full - c.alone) * filled / c.slots) + c.round;
+    if (us < least) {
+      least = us;
+      best = t;
+    }
   }
+  return best;
+}
+
+template <class F>
+void ns_with_tile(int t, F f) {
+  if (t == 0) f(Tile64());
+  else if (t == 1) f(Tile128());
+  else if (t == 2) f(Tile192());
+  else f(Tile256());
+}
+
+template <int KIND>
+void ns_sym(const NsArgs& p, int tile, int blocks, int ls, int rs, int ds, hipStream_t st) {
+  ns_with_tile(tile, [&](auto c) {
+    using C = decltype(c);
+    ns_sym_kernel<C, KIND><<<blocks, C::THREADS, 0, st>>>(p, ls, rs, ds);
+  });
 }
 
 }  // namespace
@@ -409,37 +470,64 @@ void ns_shape(NsGroup& g) {
   g.scale = (float)std::sqrt(std::max(1.0, (double)g.rows / g.cols));
 }
 
-int64_t ns_ws_elements(const NsGroup& g) { return g.count * (6 * (int64_t)g.mp * g.np + 2 * kSlots * (int64_t)g.mp * g.mp); }
+int64_t ns_ws_elements(const NsGroup& g) { return g.count * ns_stride(g); }
 
 void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const NsUpdate& u, int steps, uint16_t* ws,
             double* part, hipStream_t st) {
-  using C = Tile64;
   NsArgs p = {};
   p.ng = ng;
   p.ws = ws;
   p.part = part;
   std::copy(off, off + nmats, p.off);
-  int64_t at = 0;
-  int first = 0, ew = 0, init = 0, sym = 0, rect = 0;
+  int at = 0;
   for (int k = 0; k < ng; ++k) {
-    NsGroup& g = p.g[k] = groups[k];
-    const int mt = (g.mp + C::BA - 1) / C::BA, nt = (g.np + C::BA - 1) / C::BA;
-    g.first = first;
-    g.ws = at;
+    p.g[k] = groups[k];
+    p.g[k].first = at;
+    at += groups[k].count;
+  }
+  // long products first
+  std::stable_sort(p.g, p.g + ng, [](const NsGroup& a, const NsGroup& b) {
+    return a.np != b.np ? a.np > b.np : a.mp > b.mp;
+  });
+  const int tg = ns_pick(p.g, ng, kLaunchGram), ts = ns_pick(p.g, ng, kLaunchSym), tr = ns_pick(p.g, ng, kLaunchRect);
+  int ew = 0, init = 0, gram = 0, sym = 0, rect = 0;
+  int64_t wat = 0;
+  for (int k = 0; k < ng; ++k) {
+    NsGroup& g = p.g[k];
+    g.ws = wat;
     g.ew = ew;
     g.init = init;
+    g.gram = gram;
     g.sym = sym;
     g.rect = rect;
-    first += g.count;
-    at += ns_ws_elements(g);
+    wat += ns_ws_elements(g);
     ew += g.count * g.parts;
     init += g.count * (g.mp / 64) * (g.np / 64);
-    sym += g.count * mt * (mt + 1) / 2;
-    rect += g.count * mt * nt;
+    gram += ns_tiles(g, kNsTiles[tg].size, kLaunchGram);
+    sym += ns_tiles(g, kNsTiles[ts].size, kLaunchSym);
+    rect += ns_tiles(g, kNsTiles[tr].size, kLaunchRect);
   }
   ns_norm_kernel<<<ew, 256, 0, st>>>(p, u);
   ns_init_kernel<<<init, 256, 0, st>>>(p, u);
-  ns_chain<C>(p, u, steps, sym, rect, st);
+  int ver = 0;
+  for (int done = 0; done < steps; ver ^= 1) {
+    int q = kP0;
+    ns_sym<kGram>(p, tg, gram, 0, 0, kA, st);
+    ns_sym<kPoly>(p, ts, sym, kA, kA, kP0, st);
+    if (steps - done >= 2) {
+      ns_sym<kMul>(p, ts, sym, kP0, kA, kT, st);
+      ns_sym<kMul>(p, ts, sym, kT, kP0, kA, st);
+      ns_sym<kPoly>(p, ts, sym, kA, kA, kP1, st);
+      ns_sym<kMul>(p, ts, sym, kP1, kP0, kQ, st);
+      q = kQ;
+    }
+    done += q == kQ ? 2 : 1;
+    ns_with_tile(tr, [&](auto c) {
+      using C = decltype(c);
+      if (done < steps) ns_apply_kernel<C, false><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
+      else ns_apply_kernel<C, true><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
+    });
+  }
 }
 
 }  // namespace mxr
