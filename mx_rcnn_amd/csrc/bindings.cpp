@@ -848,8 +848,9 @@ Tensor int8_matmul(const Tensor& x, const Tensor& xs, const Tensor& w, const Ten
   a.code = (int)code;
   a.relu = relu;
   const int64_t bytes = mxr::int8_matmul_ws(a);
-  Tensor ws_buf = at::empty({bytes}, x.options().dtype(at::kByte));
-  mxr::int8_matmul(a, ws_buf.data_ptr(), cur_stream());
+  Tensor ws_buf;
+  if (bytes > 0) ws_buf = at::empty({bytes}, x.options().dtype(at::kByte));
+  mxr::int8_matmul(a, bytes > 0 ? ws_buf.data_ptr() : nullptr, cur_stream());
   LAUNCH_CHECK("int8_matmul");
   return y;
 }

@@ -10,6 +10,7 @@
 #include "tile_nt.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mxr {
 namespace {
@@ -69,22 +70,144 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
 }
 
 // ---- products -----------------------------------------------------------------------------------
-// Rows to a 16-byte-aligned copy, `lda` bytes apart, zeros behind K.
-__global__ void __launch_bounds__(256) pack_rows_kernel(const int8_t* __restrict__ x, int64_t ld_, int K,
-                                                        int8_t* __restrict__ y, int lda) {
-  const int8_t* src = x + (int64_t)blockIdx.x * ld_;
-  int8_t* dst = y + (int64_t)blockIdx.x * lda;
-  for (int k = threadIdx.x * 4; k < lda; k += 1024) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w |= k + e < K ? (uint32_t)(uint8_t)src[k + e] << (8 * e) : 0u;
-    *reinterpret_cast<uint32_t*>(dst + k) = w;
-  }
+// 16 bytes at any address: the compiler's unaligned load (one instruction on this target)
+__device__ __forceinline__ uint4 load16(const int8_t* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// bytes k .. k + 15 of a row of K, zeros behind its end; nothing behind it is read
+__device__ __forceinline__ uint4 load16_tail(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return load16(row + k);
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int e = 0; e < K - k; ++e) w[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Both operands' rows to 16-byte-aligned copies, `lda` bytes apart, zeros behind K: those of w follow those of x.
+__global__ void __launch_bounds__(256) pack_rows_kernel(Int8Args p, int8_t* __restrict__ y, int lda) {
+  const int64_t row = blockIdx.x;
+  const int8_t* src = row < p.M ? p.x + row * p.ldx : p.w + (row - p.M) * p.ldw;
+  for (int k = threadIdx.x * 16; k < lda; k += 4096)
+    *reinterpret_cast<uint4*>(y + row * lda + k) = load16_tail(src, k, p.K);
 }
 
 __device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bias, int relu) {
   const float v = (float)acc * xs * ws + bias;
   return relu && v < 0.f ? 0.f : v;  // (a NaN stays)
+}
+
+// Four outputs n .. n + 3 of row m: the result, or with several runs of K the run's int32 sums.
+__device__ __forceinline__ void int8_store(const Int8Args& p, int32_t* part, int splits, int sp, int64_t m, int n,
+                                           const nt_i32x4& acc) {
+  if (m >= p.M || n >= p.N) return;
+  const int cnt = min(4, p.N - n);
+  const bool vec = cnt == 4 && p.N % 4 == 0;
+  if (splits > 1) {
+    int32_t* d = part + ((int64_t)sp * p.M + m) * p.N + n;
+    if (vec) *reinterpret_cast<int4*>(d) = make_int4(acc[0], acc[1], acc[2], acc[3]);
+    else
+      for (int e = 0; e < cnt; ++e) d[e] = acc[e];
+    return;
+  }
+  const float xs = p.xs[m];
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = min(n + e, p.N - 1);
+    v[e] = int8_out(acc[e], xs, p.ws[c], p.bias != nullptr ? p.bias[c] : 0.f, p.relu);
+  }
+  const int64_t at = m * p.N + n;
+  if (vec) st4c(p.y, at, p.code, 0, v);
+  else
+    for (int e = 0; e < cnt; ++e) st(p.y, at + e, v[e], p.code);
+}
+
+// Few rows of x, or little of everything: each of KG waves reads both operands' fragments of every KG-th K tile
+// straight into registers, two K tiles ahead, with no barrier until the sums of the waves are added up in LDS.  A
+// block has 16 rows of w and 16 TB rows of x, and does without a copy of unaligned rows.  One row against 4096 x 25088:
+// 19.5 us, 5.3 TB/s.
+template <int TB, bool ALIGNED>
+struct Int8Stream {
+  static constexpr int KG = 8, U = 2;
+  const Int8Args& p;
+  int n0, k_hi, r, ch, kg;
+  int64_t m0;
+  __amdgpu_buffer_rsrc_t rw, rx;
+  uint32_t ow, ox[TB];
+
+  __device__ __forceinline__ Int8Stream(const Int8Args& a, int n, int64_t m, int k)
+      : p(a), n0(n), k_hi(k), r(threadIdx.x & 15), ch((threadIdx.x & 63) >> 4 << 4),
+        kg(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m) {
+    const int wr = min(p.N - n0, 16), xr = (int)min(p.M - m0, (int64_t)16 * TB);
+    const int ldw = (int)p.ldw, ldx = (int)p.ldx;  // (used where rows are aligned: below 2^22)
+    rw = nt_rsrc(reinterpret_cast<const char*>(p.w) + n0 * p.ldw, (wr - 1) * ldw + k_hi);
+    rx = nt_rsrc(reinterpret_cast<const char*>(p.x) + m0 * p.ldx, (xr - 1) * ldx + k_hi);
+    ow = r < wr ? (uint32_t)(r * ldw + ch) : kNtOob;
+#pragma unroll
+    for (int j = 0; j < TB; ++j) ox[j] = j * 16 + r < xr ? (uint32_t)((j * 16 + r) * ldx + ch) : kNtOob;
+  }
+  struct Frags {
+    uint4 w[U][2], x[U][2][TB];
+  };
+  __device__ __forceinline__ uint4 row16(const int8_t* base, int64_t ld_, int64_t row, int64_t rows, int k) const {
+    if (row >= rows || k >= k_hi) return make_uint4(0, 0, 0, 0);
+    return load16_tail(base + row * ld_, k, k_hi);
+  }
+  __device__ __forceinline__ void load(Frags& d, int k0) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + (u * KG + kg) * 128 + h * 64;
+        if constexpr (ALIGNED) {
+          const bool in = k + ch < k_hi;
+          d.w[u][h] = nt_load(rw, in ? ow : kNtOob, k);
+#pragma unroll
+          for (int j = 0; j < TB; ++j) d.x[u][h][j] = nt_load(rx, in ? ox[j] : kNtOob, k);
+        } else {
+          d.w[u][h] = row16(p.w, p.ldw, n0 + r, p.N, k + ch);
+#pragma unroll
+          for (int j = 0; j < TB; ++j) d.x[u][h][j] = row16(p.x, p.ldx, m0 + j * 16 + r, p.M, k + ch);
+        }
+      }
+  }
+  static __device__ __forceinline__ void mma(const Frags& d, nt_i32x4 (&acc)[TB]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TB; ++j) acc[j] = nt_mma(d.w[u][h], d.x[u][h][j], acc[j]);
+  }
+};
+
+template <int TB, bool ALIGNED>
+__global__ void __launch_bounds__(512) int8_stream_kernel(Int8Args p, int nt, int mt) {
+  using S = Int8Stream<TB, ALIGNED>;
+  __shared__ nt_i32x4 sums[S::KG][TB][64];
+  const int id = nt_xcd_item(blockIdx.x, nt * mt), lane = threadIdx.x & 63;
+  const S s(p, id / mt * 16, (int64_t)(id % mt) * 16 * TB, p.K);
+  constexpr int STEP = S::U * S::KG * 128;
+  nt_i32x4 acc[TB];
+#pragma unroll
+  for (int j = 0; j < TB; ++j) acc[j] = nt_i32x4{0, 0, 0, 0};
+  typename S::Frags f[2];
+  s.load(f[0], 0);
+  for (int k = 0; k < p.K; k += 2 * STEP) {  // (K tiles past the end are zeros)
+    s.load(f[1], k + STEP);
+    S::mma(f[0], acc);
+    s.load(f[0], k + 2 * STEP);
+    S::mma(f[1], acc);
+  }
+#pragma unroll
+  for (int j = 0; j < TB; ++j) sums[s.kg][j][lane] = acc[j];
+  __syncthreads();
+  if (s.kg >= TB) return;
+  nt_i32x4 t = sums[0][s.kg][lane];
+#pragma unroll
+  for (int g = 1; g < S::KG; ++g) t += sums[g][s.kg][lane];
+  int8_store(p, nullptr, 1, 0, s.m0 + s.kg * 16 + s.r, s.n0 + s.ch / 4, t);
 }
 
 // One BA (of N) x BB (of M) tile and one run of K per block: the result itself, or with several runs the
@@ -111,66 +234,119 @@ __global__ void __launch_bounds__(C::THREADS) int8_tile_kernel(Int8Args p, int n
       if (!C::mine(i, j)) continue;
       const int n = n0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;
       const int64_t m = m0 + (wb * C::TB + j) * 16 + (lane & 15);
-      if (m >= p.M || n >= p.N) continue;
-      const int cnt = min(4, p.N - n);
-      if (splits > 1) {
-        int32_t* d = part + ((int64_t)sp * p.M + m) * p.N + n;
-        if (cnt == 4 && p.N % 4 == 0) *reinterpret_cast<int4*>(d) = make_int4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-        else
-          for (int e = 0; e < cnt; ++e) d[e] = acc[i][j][e];
-        continue;
-      }
-      const float xs = p.xs[m];
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = min(n + e, p.N - 1);
-        v[e] = int8_out(acc[i][j][e], xs, p.ws[c], p.bias != nullptr ? p.bias[c] : 0.f, p.relu);
-      }
-      const int64_t at = m * p.N + n;
-      if (cnt == 4 && p.N % 4 == 0) st4c(p.y, at, p.code, 0, v);
-      else
-        for (int e = 0; e < cnt; ++e) st(p.y, at + e, v[e], p.code);
+      int8_store(p, part, splits, sp, m, n, acc[i][j]);
     }
 }
 
 __global__ void __launch_bounds__(256) int8_join_kernel(Int8Args p, int splits, const int32_t* __restrict__ part) {
   const int64_t total = p.M * p.N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    int acc = 0;
-    for (int s = 0; s < splits; ++s) acc += part[s * total + i];
-    const int64_t m = i / p.N;
-    const int n = (int)(i - m * p.N);
-    st(p.y, i, int8_out(acc, p.xs[m], p.ws[n], p.bias != nullptr ? p.bias[n] : 0.f, p.relu), p.code);
+  const bool vec = p.N % 4 == 0;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += (int64_t)gridDim.x * 1024) {
+    nt_i32x4 acc = {0, 0, 0, 0};
+    if (vec) {
+      for (int s = 0; s < splits; ++s) acc += *reinterpret_cast<const nt_i32x4*>(part + s * total + i);
+      const int64_t m = i / p.N;
+      int8_store(p, nullptr, 1, 0, m, (int)(i - m * p.N), acc);
+    } else {
+      for (int64_t e = i; e < min(i + 4, total); ++e) {
+        int a = 0;
+        for (int s = 0; s < splits; ++s) a += part[s * total + e];
+        const int64_t m = e / p.N;
+        const int n = (int)(e - m * p.N);
+        st(p.y, e, int8_out(a, p.xs[m], p.ws[n], p.bias != nullptr ? p.bias[n] : 0.f, p.relu), p.code);
+      }
+    }
   }
 }
 
-using Int8Tile = NtCfg<false, 64, 64, 1, 2, 2, 4>;
+// ---- choice of kernel ---------------------------------------------------------------------------
+// Tiles and their measured cost: microseconds per K tile of 128 bytes with up to half of the slots (blocks resident on
+// the chip) taken and with all, and per round (start, epilogue).  Runs of K summed apart cost a second launch and
+// their traffic.  Measured, us: 300 x 4096 x 25088 in 4 runs of 128 x 160 tiles 50, in 8 of 256 x 160 56, in 5 of 128 x 128
+// 55, in 8 of 256 x 256 60; 2400 x 4096 x 25088 258 with 256 x 160 (1.9 POPS), 264 256 x 256 (3 runs), 295 128 x 160, 569
+// 64 x 64; 64 x 4096 x 25088 25 in 4 runs of 64 x 64, 28 in 8 of 128 x 160.
+using Int8Tile64 = NtCfg<false, 64, 64, 1, 2, 2, 4>;
+using Int8Tile128 = NtCfg<false, 128, 160, 1, 4, 2, 4>;  // (a ring of 4 fills the LDS)
+using Int8Tile256 = NtCfg<false, 256, 160, 1, 4, 2, 2>;
+
+struct Int8Cand {
+  int bn, bm, slots;
+  double half, full, round;
+};
+constexpr Int8Cand kInt8Tiles[3] = {
+    {64, 64, 512, 0.35, 0.60, 2.5}, {128, 160, 256, 0.63, 0.80, 4.0}, {256, 160, 256, 1.00, 1.28, 6.0}};
 
 struct Int8Plan {
+  int kind;  // 0, 1: stream of 16 / 32 rows of x, 2 ..: tiles
   bool pack;
   int lda, nt, mt, splits, run;
   int64_t pack_bytes, bytes;
+  double us;
 };
 
-Int8Plan int8_plan(const Int8Args& a) {
-  using C = Int8Tile;
-  Int8Plan p;
+bool int8_aligned(const void* q, int64_t ld) {
   // 16-byte loads, and 32-bit offsets within a tile's rows
-  const auto aligned = [](const void* q, int64_t ld) {
-    return (reinterpret_cast<uintptr_t>(q) | (uint64_t)ld) % 16 == 0 && ld < (1 << 22);
-  };
-  p.pack = a.K % 16 != 0 || !aligned(a.x, a.ldx) || !aligned(a.w, a.ldw);
-  p.lda = (a.K + 15) / 16 * 16;
-  p.nt = div_up(a.N, C::BA);
-  p.mt = div_up(a.M, C::BB);
-  const int nk = div_up(p.lda, 128);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ((int64_t)p.nt * p.mt), nk / 8));
-  p.run = std::max(1, div_up(nk, p.splits)) * 128;
-  p.splits = std::max(1, div_up(nk * 128, p.run));
-  p.pack_bytes = p.pack ? ((a.M + a.N) * p.lda + 255) / 256 * 256 : 0;
-  p.bytes = p.pack_bytes + (p.splits > 1 ? p.splits * a.M * a.N * 4 : 0);
-  return p;
+  return (reinterpret_cast<uintptr_t>(q) | (uint64_t)ld) % 16 == 0 && ld < (1 << 22);
+}
+
+Int8Plan int8_plan(const Int8Args& a) {
+  Int8Plan best = {};
+  best.us = 1e30;
+  const bool aligned = a.K % 16 == 0 && int8_aligned(a.x, a.ldx) && int8_aligned(a.w, a.ldw);
+  const int lda = (a.K + 15) / 16 * 16, nk = std::max(1, div_up(lda, 128));
+  const double mn = (double)a.M * a.N, k = a.K;
+  const double hbm = ((double)a.N + a.M) * k / 5.2e6;
+  const double pack_us = aligned ? 0 : 4 + 2 * (a.M + a.N) * k / 3e6;
+  const int64_t pack_bytes = aligned ? 0 : ((a.M + a.N) * lda + 255) / 256 * 256;
+  for (int s = 0; s < 4; ++s) {  // 16 or 32 rows of x; unaligned rows as they are, or copied first
+    if (s >= 2 && aligned) break;
+    Int8Plan p = {};
+    p.kind = s & 1;
+    p.pack = s >= 2;
+    p.lda = lda;
+    p.nt = div_up(a.N, 16);
+    p.mt = div_up(a.M, 16 << p.kind);
+    p.splits = 1;
+    const double blocks = (double)p.nt * p.mt, rows = std::min<double>(a.M, 16 << p.kind);
+    p.us = std::max(hbm, std::ceil(blocks / 512) * (std::ceil(nk / 16.0) * (aligned || p.pack ? 0.9 : 4.5) + 2)) +
+           blocks * (rows + (p.mt > 1 ? 16 : 0)) * k / 12e6 + 2;
+    if (p.pack) {
+      p.us += pack_us;
+      p.pack_bytes = p.bytes = pack_bytes;
+    }
+    if (blocks < 2147483647.0 && p.us < best.us) best = p;
+  }
+  for (int t = 0; t < 3; ++t) {
+    const Int8Cand& c = kInt8Tiles[t];
+    for (int splits : {1, 2, 3, 4, 6, 8, 12}) {
+      Int8Plan p = {};
+      p.kind = 2 + t;
+      p.pack = !aligned;
+      p.lda = lda;
+      p.nt = div_up(a.N, c.bn);
+      p.mt = div_up(a.M, c.bm);
+      const int run = div_up(nk, splits);
+      p.run = run * 128;
+      p.splits = div_up(nk, run);
+      if (p.splits != splits) continue;
+      const double blocks = (double)p.nt * p.mt * splits, whole = std::floor(blocks / c.slots);
+      const double rest = blocks - whole * c.slots;
+      p.us = whole * (run * c.full + c.round) + 2;
+      if (rest > 0) p.us += run * (c.half + (c.full - c.half) * std::max(0.0, 2 * rest / c.slots - 1)) + c.round;
+      p.us = std::max(p.us, hbm);
+      if (splits > 1) p.us += 3 + splits * mn * 8 / 6e6;
+      p.us += pack_us;
+      p.pack_bytes = pack_bytes;
+      p.bytes = pack_bytes + (splits > 1 ? splits * a.M * a.N * 4 : 0);
+      if (blocks < 2147483647.0 && p.us < best.us) best = p;
+    }
+  }
+  return best;
+}
+
+template <class C>
+void int8_tiles(const Int8Args& a, const Int8Plan& p, int32_t* part, hipStream_t st) {
+  int8_tile_kernel<C><<<(unsigned)(p.nt * p.mt * p.splits), C::THREADS, 0, st>>>(a, p.nt, p.mt, p.splits, p.run, part);
 }
 
 }  // namespace
@@ -192,23 +368,30 @@ void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int
 int64_t int8_matmul_ws(const Int8Args& a) { return int8_plan(a).bytes; }
 
 void int8_matmul(const Int8Args& args, void* ws, hipStream_t st) {
-  using C = Int8Tile;
   Int8Args a = args;
   const Int8Plan p = int8_plan(a);
   if (p.pack) {
     int8_t* xb = static_cast<int8_t*>(ws);
-    int8_t* wb = xb + a.M * p.lda;
-    pack_rows_kernel<<<(unsigned)a.M, 256, 0, st>>>(a.x, a.ldx, a.K, xb, p.lda);
-    pack_rows_kernel<<<(unsigned)a.N, 256, 0, st>>>(a.w, a.ldw, a.K, wb, p.lda);
+    pack_rows_kernel<<<(unsigned)(a.M + a.N), 256, 0, st>>>(a, xb, p.lda);
     a.x = xb;
-    a.w = wb;
+    a.w = xb + a.M * p.lda;
     a.ldx = a.ldw = a.K = p.lda;
   }
+  if (p.kind < 2) {
+    const bool aligned = a.K % 16 == 0 && int8_aligned(a.x, a.ldx) && int8_aligned(a.w, a.ldw);
+    const unsigned grid = (unsigned)(p.nt * p.mt);
+    if (p.kind == 0 && aligned) int8_stream_kernel<1, true><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
+    else if (p.kind == 0) int8_stream_kernel<1, false><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
+    else if (aligned) int8_stream_kernel<2, true><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
+    else int8_stream_kernel<2, false><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
+    return;
+  }
   int32_t* part = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + p.pack_bytes);
-  const int64_t grid = (int64_t)p.nt * p.mt * p.splits;
-  int8_tile_kernel<C><<<(unsigned)grid, C::THREADS, 0, st>>>(a, p.nt, p.mt, p.splits, p.run, part);
+  if (p.kind == 2) int8_tiles<Int8Tile64>(a, p, part, st);
+  else if (p.kind == 3) int8_tiles<Int8Tile128>(a, p, part, st);
+  else int8_tiles<Int8Tile256>(a, p, part, st);
   if (p.splits > 1)
-    int8_join_kernel<<<(unsigned)std::min<int64_t>(div_up(a.M * a.N, 256), 4096), 256, 0, st>>>(a, p.splits, part);
+    int8_join_kernel<<<(unsigned)std::min<int64_t>(div_up(a.M * a.N, 1024), 4096), 256, 0, st>>>(a, p.splits, part);
 }
 
 }  // namespace mxr

@@ -51,12 +51,14 @@ struct NtCfg {
   static constexpr int GROUP = WA * WB, WAVES = KG * GROUP, THREADS = 64 * WAVES;
   static constexpr int TA = BA / WA / 16, TB = BB / WB / 16;
   static constexpr int ROWS = BA + BB;               // LDS rows of a K tile: A, then B
-  static constexpr int LPT = KG * ROWS / 8 / WAVES;  // DMA instructions (8 rows) of a wave per stage
-  static constexpr int TILE = ROWS * 128, STAGE = KG * TILE, RING = NR * STAGE;
+  // DMA instructions (8 rows) of a wave per stage; where they come out uneven (int8 only), the last ones fill rows
+  // behind the stage's that nobody reads
+  static constexpr int LPT = (KG * ROWS / 8 + WAVES - 1) / WAVES;
+  static constexpr int TILE = ROWS * 128, STAGE = LPT * WAVES * 1024, RING = NR * STAGE;
   static constexpr int JOIN = KG > 1 ? WAVES * TA * TB * 1024 : 0;  // accumulators exchanged between groups
   static constexpr int LDS = RING > JOIN + WAVES * 1280 ? RING : JOIN + WAVES * 1280;
   using Acc = typename std::conditional<PAIR, nt_f32x4, nt_i32x4>::type;
-  static_assert(KG * ROWS % (8 * WAVES) == 0, "every wave issues the same number of 8-row loads");
+  static_assert(!PAIR || KG * ROWS % (8 * WAVES) == 0, "pairs: every load has its rows");
   static_assert(BA % (16 * WA) == 0 && BB % (16 * WB) == 0, "whole 16x16 tiles per wave");
   static_assert(NR >= 2 && LDS <= 160 * 1024 && (NR - 1) * LPT < 64, "ring depth (vmcnt counts to 63)");
   // this wave: its group, its place in it; the 16 x 16 tiles that it holds after the join
@@ -86,6 +88,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t nt_rsrc(const char* base, int 
 // 16 bytes per lane from byte `voff` + `soff` of the window to 1 KiB of LDS, lane after lane
 __device__ __forceinline__ void nt_dma(__amdgpu_buffer_rsrc_t rs, char* lds, uint32_t voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, (int)voff, soff, 0, 0);
+}
+
+// the same 16 bytes into registers
+typedef uint32_t nt_u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 nt_load(__amdgpu_buffer_rsrc_t rs, uint32_t voff, int soff) {
+  return __builtin_bit_cast(uint4, (nt_u32x4)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)voff, soff, 0));
 }
 
 __device__ __forceinline__ nt_f32x4 nt_mma(const uint4& a, const uint4& b, nt_f32x4 c) {
@@ -194,7 +202,7 @@ __device__ __forceinline__ void nt_loop_body(char* lds, const char* __restrict__
       off[i] = row * 128 + chunk[i];
     } else {
       chunk[i] += g * 128;
-      off[i] = row < (is_b ? brows : arows) ? (uint32_t)row * (is_b ? B.ld : A.ld) + (uint32_t)chunk[i] : kNtOob;
+      off[i] = g < C::KG && row < (is_b ? brows : arows) ? (uint32_t)row * (is_b ? B.ld : A.ld) + (uint32_t)chunk[i] : kNtOob;
     }
   }
   // int8: one window per operand, up to the end of its last row

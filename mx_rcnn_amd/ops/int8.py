@@ -25,14 +25,11 @@ def quantize_rows(x):
     """(M, K) fp32 / bf16 / fp16 -> (int8 (M, K), fp32 scales (M,)): scale = max|row| * (1 / 127) in fp32
     (at least 2^-126), values divided by it and rounded to the nearest integer, ties to even, so that ``q * scale`` stands for the row.
     A row that holds an infinity or a NaN gets the scale NaN and zeros: what is computed from it is NaN."""
+    if x.is_cuda:
+        return tuple(need_ext().quantize_rows(_rows(x)))
     _check_float(x, 'quantize_rows')
     if x.dim() != 2:
         raise ValueError('quantize_rows: (M, K), not %s' % (tuple(x.shape),))
-    if x.is_cuda:
-        if x.shape[1] > 1 and x.stride(1) != 1:
-            x = x.contiguous()
-        q, s = need_ext().quantize_rows(x)
-        return q, s
     xf = x.float()
     peak = xf.abs().amax(1) if x.shape[1] else xf.new_zeros(x.shape[0])
     bad = ~torch.isfinite(peak)
@@ -42,6 +39,11 @@ def quantize_rows(x):
     return q, torch.where(bad, torch.full_like(s, float('nan')), s)
 
 
+def _rows(t):
+    """``t`` with its columns contiguous (its rows any stride apart)."""
+    return t if t.dim() != 2 or t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
 def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16):
     """``relu(xs[:, None] * ws * (xq @ wq.T) + bias)`` of int8 ``xq`` (M, K) and ``wq`` (N, K) with fp32
     scales ``xs`` (M,) and ``ws`` (N,) and fp32 ``bias`` (N,): the sum exact in int32 (K <= 131071), the
@@ -49,25 +51,21 @@ def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16)
     K, strides and addresses that are multiples of 16 bytes are read in place, others through a copy."""
     if out_dtype not in OUT_CODES:
         raise TypeError('int8_matmul: out_dtype fp32, bf16 or fp16, not %s' % (out_dtype,))
+    if xq.dim() == 2 and xq.shape[1] > MAX_K:
+        raise ValueError('int8_matmul: K = %d (int32 sums are exact up to %d)' % (xq.shape[1], MAX_K))
+    if xq.is_cuda:  # (the extension checks the rest)
+        return need_ext().int8_matmul(_rows(xq), xs, _rows(wq), ws, bias, relu, OUT_CODES[out_dtype])
     for t, what in ((xq, 'xq'), (wq, 'wq')):
         if t.dtype != torch.int8 or t.dim() != 2:
             raise TypeError('int8_matmul: %s must be a 2-D int8 tensor, not %s %s' % (what, t.dtype, tuple(t.shape)))
     M, K, N = xq.shape[0], xq.shape[1], wq.shape[0]
     if wq.shape[1] != K:
         raise ValueError('int8_matmul: K differs: xq %s, wq %s' % (tuple(xq.shape), tuple(wq.shape)))
-    if K > MAX_K:
-        raise ValueError('int8_matmul: K = %d (int32 sums are exact up to %d)' % (K, MAX_K))
-    vecs = [(xs, M, 'xs'), (ws, N, 'ws')] + ([] if bias is None else [(bias, N, 'bias')])
-    for t, n, what in vecs:
+    for t, n, what in [(xs, M, 'xs'), (ws, N, 'ws')] + ([] if bias is None else [(bias, N, 'bias')]):
         if t.dtype != torch.float32 or tuple(t.shape) != (n,):
             raise TypeError('int8_matmul: %s must be fp32 (%d,), not %s %s' % (what, n, t.dtype, tuple(t.shape)))
-    for t in [wq] + [v[0] for v in vecs]:
         if t.device != xq.device:
             raise ValueError('int8_matmul: tensors on %s and %s' % (xq.device, t.device))
-    if xq.is_cuda:
-        rows = [t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous() for t in (xq, wq)]
-        return need_ext().int8_matmul(rows[0], xs.contiguous(), rows[1], ws.contiguous(),
-                                      None if bias is None else bias.contiguous(), bool(relu), OUT_CODES[out_dtype])
     y = (xq.to(torch.int32) @ wq.to(torch.int32).t()).float()
     y = y * xs[:, None] * ws
     if bias is not None:
