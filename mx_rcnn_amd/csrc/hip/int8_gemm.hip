@@ -22,51 +22,135 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 __device__ __forceinline__ float row_scale(uint32_t peak) {
   return peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(peak) * (1.f / 127.f), 0x1p-126f);
 }
-__device__ __forceinline__ int to_i8(float v, float s) {
-  return (int)rintf(v / s);  // |v| <= 127 s (1 + 2^-22): never past 127
+// Eight values as they lie in memory: 8 x fp32 or 8 x 16 bits.
+template <int CODE>
+struct Raw8 {
+  uint32_t w[CODE == 0 ? 8 : 4];
+  // from any address, by the compiler's unaligned loads
+  __device__ __forceinline__ void load(const void* x, int64_t i) {
+    __builtin_memcpy(w, static_cast<const char*>(x) + i * (CODE == 0 ? 4 : 2), sizeof(w));
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if (CODE == 0) return __uint_as_float(w[e]);
+    if (CODE == 1) return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    return f16_to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+  }
+};
+
+// Eight quotients v / s rounded to integers, packed.  A quotient is taken as v * (1 / s), which is within
+// 127 * 1.5 * 2^-23 of the fp32 quotient (two roundings against one): only where that lies within 127 * 2^-22 of a tie
+// can the two round differently, and only there it is divided.  Adding 1.5 * 2^23 rounds to an integer, ties to even,
+// and leaves it in the low bits.  (|v| <= 127 s (1 + 2^-22): never past 127.)
+template <int CODE>
+__device__ __forceinline__ uint2 to_i8x8(const Raw8<CODE>& v, float s, float inv) {
+  constexpr float kBig = 12582912.f;
+  uint32_t q[8];
+  float off = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = v.get(e) * inv, r = t + kBig;
+    off = fmaxf(off, fabsf(t - (r - kBig)));
+    q[e] = __float_as_uint(r);
+  }
+  if (off > 0.5f - 127.f * 0x1p-22f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(v.get(e) / s + kBig);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(q[4 * h + 1], q[4 * h], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(q[4 * h + 3], q[4 * h + 2], 0x0c0c0400u);
+    w[h] = lo | (hi << 16);
+  }
+  return make_uint2(w[0], w[1]);
 }
 
-// One block per row; the second read of the row comes from the caches.
-template <int CODE, bool VEC>
-__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int64_t ld_, int K,
-                                                       int8_t* __restrict__ q, float* __restrict__ scale) {
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
+// T threads per row (a wave: four rows per block), which hold it in registers while its peak is found -- NV times eight
+// values each -- so that x is read once; HELD = false: a row longer than that is read twice, the second time from the
+// caches.  Rows have at least eight values: a thread whose eight would pass the end takes the last eight, and writes
+// what its neighbour writes.
+template <int CODE, int T, int NV, bool HELD>
+__global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void* __restrict__ x, int64_t ld_, int64_t rows,
+                                                                     int K, int8_t* __restrict__ q,
+                                                                     float* __restrict__ scale) {
+  const int tid = threadIdx.x % T;
+  const int64_t row = (int64_t)blockIdx.x * (T < 256 ? 256 / T : 1) + threadIdx.x / T;
+  if (row >= rows) return;  // (whole waves: rows share a block only where a row is a wave)
+  const int64_t x0 = row * ld_;
+  int8_t* out = q + row * K;
+  Raw8<CODE> v[HELD ? NV : 1];
   uint32_t peak = 0;
-  const int64_t x0 = row * ld_, q0 = row * K;
-  if (VEC) {
-    for (int k = tid * 8; k < K; k += 2048) {
-      float v[8];
-      ld8c(x, x0 + k, CODE, 0, v);
+  if constexpr (HELD) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(v[e]));
-    }
+    for (int c = 0; c < NV; ++c) v[c].load(x, x0 + min((c * T + tid) * 8, K - 8));
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(v[c].get(e)));
   } else {
-    for (int k = tid; k < K; k += 256) peak = max(peak, abs_bits(ld(x, x0 + k, CODE)));
+    for (int k = tid * 8; k < K; k += T * 8) {
+      v[0].load(x, x0 + min(k, K - 8));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(v[0].get(e)));
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) peak = max(peak, (uint32_t)__shfl_xor((int)peak, o, 64));
-  __shared__ uint32_t red[4];
-  if ((tid & 63) == 0) red[tid >> 6] = peak;
-  __syncthreads();
-  peak = max(max(red[0], red[1]), max(red[2], red[3]));
-  const float s = row_scale(peak);
-  if (tid == 0) scale[row] = s;
-  const bool bad = s != s;
-  if (VEC) {
-    for (int k = tid * 8; k < K; k += 2048) {
-      float v[8];
-      ld8c(x, x0 + k, CODE, 0, v);
-      uint32_t w[2] = {0, 0};
-      if (!bad) {
+  if constexpr (T > 64) {
+    __shared__ uint32_t red[T / 64];
+    if ((tid & 63) == 0) red[tid >> 6] = peak;
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(to_i8(v[e], s) & 255) << (8 * (e & 3));
-      }
-      *reinterpret_cast<uint2*>(q + q0 + k) = make_uint2(w[0], w[1]);
-    }
-  } else {
-    for (int k = tid; k < K; k += 256) q[q0 + k] = bad ? 0 : (int8_t)to_i8(ld(x, x0 + k, CODE), s);
+    for (int w = 0; w < T / 64; ++w) peak = max(peak, red[w]);
   }
+  const float s = row_scale(peak);
+  const bool bad = s != s;
+  const float inv = 1.f / s;
+  if (tid == 0) scale[row] = s;
+  const auto put = [&](const Raw8<CODE>& d, int k) {
+    const uint2 w = bad ? make_uint2(0, 0) : to_i8x8(d, s, inv);
+    __builtin_memcpy(out + min(k, K - 8), &w, 8);
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+      if ((c * T + tid) * 8 < K) put(v[c], (c * T + tid) * 8);
+  } else {
+    for (int k = tid * 8; k < K; k += T * 8) {
+      v[0].load(x, x0 + min(k, K - 8));
+      put(v[0], k);
+    }
+  }
+}
+
+// Rows of fewer than eight values: a thread each.
+__global__ void __launch_bounds__(256) quantize_short_kernel(const void* __restrict__ x, int code, int64_t ld_,
+                                                             int64_t rows, int K, int8_t* __restrict__ q,
+                                                             float* __restrict__ scale) {
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= rows) return;
+  uint32_t peak = 0;
+  for (int k = 0; k < K; ++k) peak = max(peak, abs_bits(ld(x, row * ld_ + k, code)));
+  const float s = row_scale(peak);
+  scale[row] = s;
+  for (int k = 0; k < K; ++k) q[row * K + k] = s != s ? 0 : (int8_t)rintf(ld(x, row * ld_ + k, code) / s);
+}
+
+template <int CODE>
+void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, float* scale, hipStream_t st) {
+  const auto go = [&](auto kernel, int t) {
+    const int per = t < 256 ? 256 / t : 1;
+    kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, scale);
+  };
+  if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, scale);
+  // 2400 x 25088 bf16 with 256 / 512 / 1024 threads per row: 36 / 33 / 41 us (512: 5.5 TB/s)
+  else if (K <= 512) go(quantize_kernel<CODE, 64, 1, true>, 64);
+  else if (K <= 2048 && rows >= 2048) go(quantize_kernel<CODE, 64, 4, true>, 64);
+  else if (K <= 4096) go(quantize_kernel<CODE, 256, 2, true>, 256);
+  else if (K <= 8192) go(quantize_kernel<CODE, 512, 2, true>, 512);
+  else if (K <= 32768) go(quantize_kernel<CODE, 512, 8, true>, 512);
+  else go(quantize_kernel<CODE, 1024, 1, false>, 1024);
 }
 
 // ---- products -----------------------------------------------------------------------------------
@@ -352,17 +436,9 @@ void int8_tiles(const Int8Args& a, const Int8Plan& p, int32_t* part, hipStream_t
 }  // namespace
 
 void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, float* scale, hipStream_t st) {
-  const int64_t esize = code == 0 ? 4 : 2;
-  const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) | (uint64_t)(ld * esize)) % 16 == 0;
-#define MXR_Q(CODE)                                                                                        \
-  do {                                                                                                     \
-    if (vec) quantize_kernel<CODE, true><<<(unsigned)rows, 256, 0, st>>>(x, ld, K, q, scale);              \
-    else quantize_kernel<CODE, false><<<(unsigned)rows, 256, 0, st>>>(x, ld, K, q, scale);                 \
-  } while (0)
-  if (code == 0) MXR_Q(0);
-  else if (code == 1) MXR_Q(1);
-  else MXR_Q(2);
-#undef MXR_Q
+  if (code == 0) quantize<0>(x, rows, ld, K, q, scale, st);
+  else if (code == 1) quantize<1>(x, rows, ld, K, q, scale, st);
+  else quantize<2>(x, rows, ld, K, q, scale, st);
 }
 
 int64_t int8_matmul_ws(const Int8Args& a) { return int8_plan(a).bytes; }
