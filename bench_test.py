@@ -37,6 +37,8 @@ def parse_args(argv=None):
     ap.add_argument('--plant', type=int, default=10,
                     help='classes whose cls_score bias is raised so random-init weights produce detections above '
                          'the 0.05 threshold (the NMS / top-k post-process then has real work); 0 = off')
+    ap.add_argument('--fc-int8', dest='fc_int8', action='store_true',
+                    help='VGG16 with bf16 / fp16: fc6 / fc7 as 8-bit products (core/detector.py)')
     return ap.parse_args(argv)
 
 
@@ -98,7 +100,7 @@ def main():
         with torch.no_grad():  # synthetic "confident" classes: softmax mass well above 0.05 on them
             model.head.cls_score.bias[1:1 + args.plant] += 6.0
     cdt = args.dtype if device.type == 'cuda' else 'fp32'
-    det = Detector(model, device, compute_dtype=cdt)
+    det = Detector(model, device, compute_dtype=cdt, fc_int8=args.fc_int8)
     dev_pool = [det._prep(x) for x in pool]
     dinfo = info.to(device)
     run = None
@@ -155,6 +157,7 @@ def main():
             'config': {'model': '%s-faster-rcnn%s' % (args.network, '-c4' if args.network.startswith('resnet') else ''), 'global_batch': world * nb, 'ims_per_gpu': nb,
                        'image_hw': [h, w],
                        'num_classes': args.num_classes, 'parallelism': 'dp%d' % world, 'exec': mode,
+                       'fc': 'int8' if args.fc_int8 else args.dtype,
                        'rpn_pre_post_nms': [config.TEST.RPN_PRE_NMS_TOP_N, config.TEST.RPN_POST_NMS_TOP_N],
                        'detections_last_image': n_det}}), flush=True)
     if os.environ.get('MXR_BENCH_DUMP_TUNE') and device.type == 'cuda':

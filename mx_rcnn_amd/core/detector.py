@@ -59,6 +59,20 @@ def _inference_copy(model, dtype):
     return out.eval()
 
 
+def _quantize_fc(model, source):
+    """The FC layers ahead of the predictors (VGG16's fc6 / fc7) of the inference copy ``model`` in 8 bits,
+    from ``source``'s weights: int8 rows with one scale per output channel, laid out once (ops/int8.py)."""
+    from ..ops.int8 import quantize_rows
+    names = [k for k in ('fc6', 'fc7') if hasattr(model.head, k)]
+    if not names:
+        raise ValueError('fc_int8: the %s head has no fully connected layers' % model.network)
+    with torch.no_grad():
+        for k in names:
+            layer, w = getattr(model.head, k), getattr(source.head, k).weight.detach().float()
+            layer.int8 = quantize_rows(layer.rows_of(w).contiguous()) + \
+                (None if layer.bias is None else getattr(source.head, k).bias.detach().float(),)
+
+
 class Detector(object):
     """Test-time runner of a FasterRCNN (reference `rcnn/detector.py:8-81`).
 
@@ -68,9 +82,13 @@ class Detector(object):
     default) or 'fp16' (BASELINE config 5's fp16 MFMA path).  On the GPU the detector runs a
     private copy of the model's weights in that precision (``self.model``); ``self.source`` is the
     model it was built from, left untouched.
+
+    fc_int8: VGG16's fc6 / fc7 run as 8-bit products -- weights one scale per output channel, quantized
+    here once, RoI rows one scale each, quantized per call; the rest of the graph keeps ``compute_dtype``
+    (on the GPU bf16 or fp16).
     """
 
-    def __init__(self, symbol, ctx=None, arg_params=None, aux_params=None, compute_dtype=None):
+    def __init__(self, symbol, ctx=None, arg_params=None, aux_params=None, compute_dtype=None, fc_int8=False):
         self.ctx = torch.device(ctx) if ctx is not None else torch.device('cpu')
         if arg_params is not None or aux_params is not None:
             from .module import MutableModule
@@ -94,6 +112,12 @@ class Detector(object):
             self.model = _inference_copy(symbol, compute_dtype)
         else:
             self.model = symbol.to(self.ctx).eval()
+        if fc_int8:
+            if self.ctx.type == 'cuda' and compute_dtype == torch.float32:
+                raise ValueError('fc_int8: with compute_dtype bf16 or fp16, not fp32')
+            if self.model is symbol:  # the CPU detector runs the model itself: 8-bit layers go on a copy
+                self.model = _inference_copy(symbol, compute_dtype)
+            _quantize_fc(self.model, symbol)
 
     def precision_scope(self):
         """Context in which this detector's model runs (the three-plane mode for GPU fp32)."""

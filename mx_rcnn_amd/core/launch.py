@@ -58,6 +58,22 @@ def add_common_args(parser, eval_cli=False):
     return parser
 
 
+def add_optimizer_args(parser):
+    parser.add_argument('--optimizer', default='sgd', choices=('sgd', 'muon'),
+                        help='sgd (the reference optimizer) or muon: conv / FC weights except the predictors step '
+                             'along their orthogonalised momentum (ops/muon.py), the rest with sgd')
+    parser.add_argument('--muon-lr-mult', dest='muon_lr_mult', type=float, default=20.0,
+                        help='learning rate of the muon matrices, as a multiple of --lr')
+    return parser
+
+
+def add_fc_int8_arg(parser):
+    parser.add_argument('--fc-int8', dest='fc_int8', action='store_true',
+                        help='VGG16 with --dtype bf16 / fp16: fc6 / fc7 as 8-bit products, one scale per RoI and '
+                             'per output channel (ops/int8.py)')
+    return parser
+
+
 def init_runtime(args):
     """Spawn the per-GPU ranks if ``--gpus`` names more than one device (the parent exits with
     the job's code and never touches the GPU), then bootstrap this rank."""
@@ -107,11 +123,14 @@ def build_model(network, num_classes, pretrained=None, load_epoch=0, resume=Fals
     return model, arg, aux
 
 
-def optimizer_params(lr, mom, wd, factor_step, resume, warmup=True):
+def optimizer_params(lr, mom, wd, factor_step, resume, warmup=True, muon_lr_mult=None):
     sched = FactorScheduler(factor_step, 0.1) if (resume or not warmup) else \
         WarmupScheduler(factor_step, 0.1, warmup_lr=0.1 * lr, warmup_step=200)
-    return {'momentum': mom, 'wd': wd, 'learning_rate': lr, 'lr_scheduler': sched, 'clip_gradient': 1.0,
-            'rescale_grad': 1.0}
+    out = {'momentum': mom, 'wd': wd, 'learning_rate': lr, 'lr_scheduler': sched, 'clip_gradient': 1.0,
+           'rescale_grad': 1.0}
+    if muon_lr_mult is not None:
+        out['muon_lr_mult'] = muon_lr_mult
+    return out
 
 
 def e2e_config():

@@ -175,7 +175,7 @@ class MutableModule(object):
     def init_optimizer(self, kvstore='device', optimizer='sgd', optimizer_params=None, force_init=False):
         if self.optimizer_initialized and not force_init:
             return
-        assert optimizer == 'sgd', 'only SGD (the reference optimizer) is implemented'
+        assert optimizer in ('sgd', 'muon'), 'sgd (the reference optimizer) or muon'
         p = dict(optimizer_params or {})
         lr = p.get('learning_rate', 0.01)
         sched = p.get('lr_scheduler')
@@ -185,7 +185,8 @@ class MutableModule(object):
                                rescale_grad=p.get('rescale_grad', 1.0), lr_scheduler=sched,
                                compute_dtype=self.compute_dtype, device=self.context,
                                bucket_mb=p.get('bucket_mb', 64),
-                               precision=self.precision if self.context.type == 'cuda' else None)
+                               precision=self.precision if self.context.type == 'cuda' else None,
+                               optimizer=optimizer, **{k: p[k] for k in ('muon_lr_mult', 'muon_momentum') if k in p})
         if self._monitor is not None:  # a norm monitor reads the gradients: no fused updates
             self.trainer.fused_fc_sgd = []
         self.optimizer_initialized = True

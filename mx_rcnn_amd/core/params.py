@@ -22,9 +22,15 @@ import os
 import torch
 import torch.nn as nn
 
+from ..ops.muon import muon_update_
 from ..ops.sgd import sgd_momentum_
 from ..ops import grad_sink
 from ..ops import precision
+
+
+# the predictors stay with SGD under the Muon optimizer: their rows are classes and box deltas, whose
+# gradients differ in size for good reason
+MUON_EXCLUDE = ('rpn_cls_score', 'rpn_bbox_pred', 'cls_score', 'bbox_pred')
 
 
 def _is_bn_param(name):
@@ -109,6 +115,8 @@ class FlatParamStore:
         self.groups = [ParamGroup(k, v, dev, compute_dtype, self.x2) for k, v in sorted(groups.items())]
         self.params = {}
         self._fused = {}  # group index -> fused-update specs (enable_fused_sgd)
+        self._muon = {}   # group index -> (element offset, rows, cols) of its Muon matrices (enable_muon)
+        self._muon_args = None
         with torch.no_grad():
             for g in self.groups:
                 off = 0
@@ -375,7 +383,8 @@ class FlatParamStore:
         kernel zeroes each group's gradient buffer after reading it (replaces zero_grad).
         Parameters whose update ran fused into their weight gradient this step
         (enable_fused_sgd), and ranges the reducer already updated after their all-reduce
-        (:meth:`mark_updated`), are skipped."""
+        (:meth:`mark_updated`), are skipped.  Matrices of :meth:`enable_muon` take their Muon update
+        (its own learning rate and momentum) in place of SGD's."""
         early = getattr(self, '_early', {})
         self._early = {}
         for gi, g in enumerate(self.groups):
@@ -384,6 +393,13 @@ class FlatParamStore:
                           early.get(id(g), []))
             for sp in self._fused.get(gi, ()):
                 sp['applied'] = False
+            mats = self._muon.get(gi, ())
+            if mats:
+                skip = sorted(skip + [(o, o + r * c) for o, r, c in mats])
+                mlr, mmom, nesterov = self._muon_args
+                muon_update_(g.master, g.mom, grad, mats, mlr, momentum=mmom, wd=wd if g.decay else 0.0,
+                             rescale=rescale, clip=clip, nesterov=nesterov, w_bf16=g.shadow, planes=g.x2 or 1,
+                             zero=g.grad if clear else None)
             if not skip:
                 sgd_momentum_(g.master, g.mom, grad, lr, momentum, wd if g.decay else 0.0, rescale, clip, g.shadow,
                               planes=g.x2 or 1, zero=g.grad if clear else None)
@@ -436,6 +452,24 @@ class FlatParamStore:
                 self._fused.setdefault(gi, []).append(spec)
                 done.append(n)
         return done
+
+    def enable_muon(self, lr, momentum=0.95, nesterov=True):
+        """Let :meth:`sgd_step` update every conv / FC weight but the predictors (MUON_EXCLUDE) along
+        its orthogonalised momentum (ops/muon.py), as the (out, in * kh * kw) matrix it is, with the learning
+        rate ``lr`` (a 1-element fp32 device tensor) and ``momentum``.  Biases, BN parameters and the
+        predictors keep SGD.  Returns the names of the matrices."""
+        assert not self._fused, 'enable_muon: weights with a fused SGD update (disable_fused_sgd first)'
+        self._muon_args = (lr, float(momentum), bool(nesterov))
+        self._muon, names = {}, []
+        for gi, g in enumerate(self.groups):
+            mats = []
+            for (n, _, _, numel, shape, cl), off in zip(g.entries, g.offsets):
+                if n.endswith('_weight') and len(shape) >= 2 and n[:-len('_weight')] not in MUON_EXCLUDE:
+                    mats.append((off, shape[0], numel // shape[0]))
+                    names.append(n)
+            if mats:
+                self._muon[gi] = tuple(mats)
+        return names
 
     def disable_fused_sgd(self):
         for specs in getattr(self, '_fused', {}).values():

@@ -18,7 +18,8 @@ from .params import FlatParamStore
 class Trainer:
     def __init__(self, model, mode='e2e', fixed_param_prefix=None, lr=0.001, momentum=0.9, wd=0.0005,
                  clip_gradient=1.0, rescale_grad=1.0, lr_scheduler=None, compute_dtype=None, device=None,
-                 bucket_mb=25, average_grads=False, channels_last=None, grad_comm_dtype=None, precision=None):
+                 bucket_mb=25, average_grads=False, channels_last=None, grad_comm_dtype=None, precision=None,
+                 optimizer='sgd', muon_lr_mult=20.0, muon_momentum=0.95):
         """precision (ops/precision.py):
         'fp32'   -- the reference's precision on the GPU: every MFMA operand and every tensor stored
                     between kernels is an EXACT (mid, hi, lo) bf16 triple of the fp32 value, products
@@ -28,7 +29,13 @@ class Trainer:
         'bf16'   -- bf16 operands, fp32 accumulation / masters;
         'torch'  -- plain fp32 PyTorch / vendor ops on the GPU (a reference arm for precision probes).
         Default: bf16 on the GPU unless compute_dtype says fp32 (then 'fp32'); the CPU path is plain
-        fp32 whatever the name."""
+        fp32 whatever the name.
+
+        optimizer: 'sgd' (the reference's), or 'muon': the conv / FC weights except the predictors step
+        along their orthogonalised momentum (ops/muon.py) at ``muon_lr_mult`` times the learning rate with
+        ``muon_momentum``, everything else with SGD as before."""
+        if optimizer not in ('sgd', 'muon'):
+            raise ValueError('optimizer must be sgd or muon, not %r' % (optimizer,))
         dev = torch.device(device) if device is not None else next(model.parameters()).device
         if precision is None:
             precision = 'fp32' if (compute_dtype == torch.float32 and dev.type == 'cuda') else 'bf16'
@@ -54,9 +61,14 @@ class Trainer:
         # VGG16's fc6 / fc7 (120 M of 137 M weights): single process, their update runs inside their
         # weight gradient (below); under data parallelism the gradient must be summed first, so their
         # buckets take the update on the reducer's optimizer stream right after their all-reduce
-        fc_names = ('fc6_weight', 'fc7_weight') if os.environ.get('MXR_FUSED_FC_SGD', '1') != '0' else ()
+        # (Muon needs the whole gradient of a matrix: no SGD fused into gradients or buckets)
+        self.optimizer = optimizer
+        fuse_fc = optimizer == 'sgd' and os.environ.get('MXR_FUSED_FC_SGD', '1') != '0'
+        fc_names = ('fc6_weight', 'fc7_weight') if fuse_fc else ()
         self.reducer = BucketReducer(self.store, bucket_mb=bucket_mb, average=average_grads,
                                      comm_dtype=grad_comm_dtype, sgd_names=fc_names)
+        if optimizer == 'muon' and self.reducer.sgd_capable:
+            raise ValueError('optimizer muon: MXR_OVERLAP_SGD updates buckets during the backward pass (SGD only)')
         if self.reducer.dp:
             self.store.broadcast_(0)  # identical starting weights on every rank
         self.momentum, self.wd, self.clip, self.rescale = momentum, wd, clip_gradient, rescale_grad
@@ -69,10 +81,15 @@ class Trainer:
         # gradient is never written, read or cleared (core/params.py enable_fused_sgd,
         # ops/vgg_fused.py); single process with the end-of-step optimizer only
         self.fused_fc_sgd = []
-        if (dev.type == 'cuda' and not self.reducer.dp and not self.reducer.sgd_capable and
-                os.environ.get('MXR_FUSED_FC_SGD', '1') != '0'):
+        if dev.type == 'cuda' and not self.reducer.dp and not self.reducer.sgd_capable and fuse_fc:
             self.fused_fc_sgd = self.store.enable_fused_sgd(('fc6_weight', 'fc7_weight'), self.lr_t, momentum, wd,
                                                             rescale_grad, clip_gradient)
+        self.muon_lr_mult = float(muon_lr_mult)
+        self.muon_lr_t = None
+        self.muon_names = []
+        if optimizer == 'muon':
+            self.muon_lr_t = torch.full((1,), float(lr) * self.muon_lr_mult, dtype=torch.float32, device=dev)
+            self.muon_names = self.store.enable_muon(self.muon_lr_t, muon_momentum)
         self.num_update = 0
         # step counter of the counter-based dropout (ops/fc.py), advanced on the device at the end
         # of every step (inside the captured graph), so a replayed graph draws a fresh mask every
@@ -249,6 +266,8 @@ class Trainer:
             lr = float(self.lr_scheduler(self.num_update))
             if lr != self._lr_set:  # a device fill only when the schedule moves
                 self.lr_t.fill_(lr)
+                if self.muon_lr_t is not None:
+                    self.muon_lr_t.fill_(lr * self.muon_lr_mult)
                 self._lr_set = lr
 
     def advance_rng(self):

@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from ..ops.bn import frozen_bn_relu, train_bn_eligible, train_bn_relu
 from ..ops.conv import conv2d
 from ..ops.fc import fully_connected, layer_seed
+from ..ops.int8 import int8_linear
 from ..ops.pool import max_pool2d
 
 
@@ -80,11 +81,16 @@ class Linear(MxLayer):
         nn.init.normal_(self.weight, 0, 0.01)
         self.rng_step = None
         self._seed = None
+        self.int8 = None  # (int8 rows, scales, fp32 bias): the weight in 8 bits, for inference (core/detector.py)
 
     def mx_arg_shapes(self):
         out = super().mx_arg_shapes()
         out['%s_weight' % self.mx_name] = (self.cout, self.cin)
         return out
+
+    def rows_of(self, w):
+        """``w`` of this layer's weight shape as the (cout, cin) rows that ``forward`` multiplies by."""
+        return w if w.dim() == 2 else w.permute(0, 2, 3, 1).reshape(w.shape[0], -1)
 
     def forward(self, x, relu=False, drop_p=0.0):
         if self.in_shape is not None:
@@ -96,12 +102,14 @@ class Linear(MxLayer):
             x = x.permute(0, 2, 3, 1).reshape(x.shape[0], -1)
         else:
             x = x.reshape(x.shape[0], -1)
+        if self.int8 is not None:
+            if self.training:
+                raise RuntimeError('%s: an 8-bit layer is for inference' % self.mx_name)
+            return int8_linear(x, *self.int8, relu=relu)
         b = None if self.bias is None else _w(self.bias, x)
         if drop_p and self.training and self._seed is None:
             self._seed = layer_seed(self.mx_name)
-        w = _w(self.weight, x)
-        if w.dim() != 2:
-            w = w.permute(0, 2, 3, 1).reshape(w.shape[0], -1)
+        w = self.rows_of(_w(self.weight, x))
         return fully_connected(x, w, b, relu, drop_p, self._seed or 0, self.rng_step, self.training)
 
 

@@ -61,9 +61,10 @@ class VGGHead(nn.Module):
             # the pooled map's channels_last rows, (h, w, c) order: a free view, matching fc6's
             # channels_last filter (Linear in_shape) -- no Flatten copy forward or backward
             rows = pooled.permute(0, 2, 3, 1).reshape(pooled.shape[0], -1)
-            if vgg_fused.head_ok(rows, self):
+            if self.fc6.int8 is None and vgg_fused.head_ok(rows, self):
                 return vgg_fused.vgg_head(rows, self)
-        x = pooled.reshape(pooled.shape[0], -1)  # MXNet Flatten: (C, H, W) order
+        # MXNet Flatten: (C, H, W) order; the 8-bit fc6 takes the map, whose channels_last rows are a view
+        x = pooled.reshape(pooled.shape[0], -1) if self.fc6.int8 is None else pooled
         # relu6/drop6 and relu7/drop7 run in the FC kernel's epilogue (ops/fc.py)
         x = self.fc6(x, relu=True, drop_p=self.dropout)
         x = self.fc7(x, relu=True, drop_p=self.dropout)

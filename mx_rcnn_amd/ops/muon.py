@@ -78,7 +78,9 @@ def muon_update_(w, mom, grad, mats, lr, momentum=0.95, wd=0.0, rescale=1.0, cli
 
     ``lr``, ``w_bf16``, ``planes``, ``plane_stride`` and ``zero`` are those of :func:`sgd_momentum_`: a
     1-element fp32 device tensor, the low-precision copy of the new weights, its planes, and the gradient
-    buffer to clear once read (the matrices' elements of it).  All matrices of a call share its launches."""
+    buffer to clear once read (the matrices' elements of it).  All matrices of a call share its launches, and
+    the tiles are chosen for the call: the same call gives the same bits, a matrix among others may end in other
+    last bits than alone."""
     _check_steps(steps, eps)
     mats = [(int(o), int(r), int(c)) for o, r, c in mats]
     for o, r, c in mats:

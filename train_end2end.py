@@ -47,8 +47,9 @@ def end2end_train(args):
     monitor = Monitor(100) if args.monitor else None
     mod.fit(train_data, eval_metric=e2e_metrics(), epoch_end_callback=do_checkpoint(args.prefix), monitor=monitor,
             batch_end_callback=Speedometer(train_data.global_batch_size, frequent=args.frequent),
-            kvstore=args.kv_store, optimizer='sgd',
-            optimizer_params=launch.optimizer_params(args.lr, args.mom, args.wd, args.factor_step, args.resume),
+            kvstore=args.kv_store, optimizer=args.optimizer,
+            optimizer_params=launch.optimizer_params(args.lr, args.mom, args.wd, args.factor_step, args.resume,
+                                                     muon_lr_mult=args.muon_lr_mult),
             arg_params=arg_params, aux_params=aux_params, begin_epoch=args.load_epoch, num_epoch=args.num_epoch,
             max_steps=args.max_steps, states_prefix=args.prefix,
             resume_states=states_file(args.pretrained, args.load_epoch) if args.resume else None)
@@ -79,6 +80,7 @@ def parse_args(argv=None):
     p.add_argument('--resume', action='store_true')
     p.add_argument('--factor-step', dest='factor_step', type=int, default=50000)
     p.add_argument('--monitor', action='store_true')
+    launch.add_optimizer_args(p)
     launch.add_common_args(p)
     return p.parse_args(argv)
 

@@ -52,9 +52,10 @@ def main(args, default_network=DEFAULT_NETWORK):
                         fixed_param_prefix=launch.FIXED_PREFIX[fam] if fam == 'resnet' else
                         ['conv1', 'conv2', 'conv3'], mode='e2e', use_graph=not args.eager)
     mod.fit(train_data, eval_metric=e2e_metrics(), epoch_end_callback=do_checkpoint(args.prefix),
-            batch_end_callback=Speedometer(args.ims_per_gpu * world, frequent=args.frequent), optimizer='sgd',
+            batch_end_callback=Speedometer(args.ims_per_gpu * world, frequent=args.frequent),
+            optimizer=args.optimizer,
             optimizer_params=launch.optimizer_params(args.lr, args.mom, args.wd, args.factor_step, args.resume,
-                                                     warmup=False),
+                                                     warmup=False, muon_lr_mult=args.muon_lr_mult),
             arg_params=arg_params, aux_params=aux_params, begin_epoch=args.load_epoch, num_epoch=args.num_epoch,
             max_steps=args.max_steps)
     pdist.destroy()
@@ -84,6 +85,7 @@ def parse_args(argv=None, default_network=DEFAULT_NETWORK):
     p.add_argument('--wd', type=float, default=0.0005)
     p.add_argument('--resume', action='store_true')
     p.add_argument('--factor-step', dest='factor_step', type=int, default=50000)
+    launch.add_optimizer_args(p)
     launch.add_common_args(p)
     a = p.parse_args(argv)
     if a.network == 'vgg16' and 'resnet' in a.pretrained:
