@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
 // per product, smaller ones fill the chip: 4096 x 4096 (us for a symmetric product / for P X) 64: 330 / 640, 128:
 // 262 / 380, 192: 222 / 410 (253 tiles, one round), 256: 265 (136 tiles on 256 CUs) / 313; ResNet-101's 84
 // matrices 64: 40 / 316, 128: 42 / 211, 192: 65 / 254, 256: 91 / 202.
-using Tile64 = NtCfg<true, 64, 64, 2, 2, 2, 2, 4, true>;  // two K groups: short products are bound by latency
+using Tile64 = NtCfg<true, 64, 64, 2, 2, 2, 4, 4, true>;  // two K groups: short products are bound by latency
 using Tile128 = NtCfg<true, 128, 128, 1, 2, 4, 2, 8>;
 using Tile192 = NtCfg<true, 192, 192, 1, 2, 4, 3, 8>;
 using Tile256 = NtCfg<true, 256, 256, 1, 2, 4, 2>;  // (no registers for sums in runs)
@@ -396,7 +396,7 @@ struct NsTile {
   double alone, full, round;
 };
 constexpr NsTile kNsTiles[4] = {
-    {64, 512, 0.33, 0.64, 5.0}, {128, 512, 0.75, 1.40, 7.0}, {192, 256, 1.31, 1.68, 9.0}, {256, 256, 1.95, 2.45, 12.0}};
+    {64, 256, 0.28, 0.30, 6.0}, {128, 512, 0.75, 1.40, 7.0}, {192, 256, 1.31, 1.68, 9.0}, {256, 256, 1.95, 2.45, 12.0}};
 
 enum NsLaunch { kLaunchGram, kLaunchSym, kLaunchRect };
 
