@@ -55,17 +55,14 @@ __device__ __forceinline__ int ns_find(const NsArgs& p, int& id, int NsGroup::*s
 // Buffers hold fp16 pairs in panels (tile_nt.h): for every 32 columns, the lines of all rows, each 32 hi and 32 lo.
 __host__ __device__ __forceinline__ int64_t ns_size(int rows, int cols) { return (int64_t)rows * cols * 2; }
 __host__ __device__ __forceinline__ int64_t ns_stride(const NsGroup& g) {  // of one matrix, in fp16 elements
-  return 3 * ns_size(g.mp, g.np) + kSlots * ns_size(g.mp, g.mp);
+  return 2 * ns_size(g.mp, g.np) + kSlots * ns_size(g.mp, g.mp);
 }
-// matrix mi of group g: X (mp x np), its transpose in two versions (np x mp), m x m slots
-__device__ __forceinline__ uint16_t* ns_x(const NsArgs& p, const NsGroup& g, int mi) {
-  return p.ws + g.ws + mi * ns_stride(g);
-}
-__device__ __forceinline__ uint16_t* ns_xt(const NsArgs& p, const NsGroup& g, int mi, int ver) {
-  return ns_x(p, g, mi) + (1 + ver) * ns_size(g.mp, g.np);
+// matrix mi of group g: X (mp x np) in two versions, m x m slots
+__device__ __forceinline__ uint16_t* ns_x(const NsArgs& p, const NsGroup& g, int mi, int ver) {
+  return p.ws + g.ws + mi * ns_stride(g) + ver * ns_size(g.mp, g.np);
 }
 __device__ __forceinline__ uint16_t* ns_sq(const NsArgs& p, const NsGroup& g, int mi, int slot) {
-  return ns_x(p, g, mi) + 3 * ns_size(g.mp, g.np) + slot * ns_size(g.mp, g.mp);
+  return ns_x(p, g, mi, 2) + slot * ns_size(g.mp, g.mp);
 }
 
 __device__ __forceinline__ void split_f16(float v, uint16_t& hi, uint16_t& lo) {
@@ -141,8 +138,8 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs p, NsUpdate u) {
   if (threadIdx.x == 0) p.part[(int64_t)(g.first + mi) * kNsParts + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Pass 2: X = u / (|u| + eps) and its transpose, as scaled fp16 pairs with zeroed padding; 64 x 64
-// elements per block, turned in LDS.  Clears the gradient it consumed when asked to.
+// Pass 2: X = u / (|u| + eps) as scaled fp16 pairs with zeroed padding; 64 x 64 elements per block, those of a tall
+// matrix turned in LDS.  Clears the gradient it consumed when asked to.
 __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
   int id = blockIdx.x;
   const int k = ns_find(p, id, &NsGroup::init);
@@ -163,6 +160,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
   __syncthreads();
   const double f = (double)kNsX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + u.eps);
   const int lr = tid >> 4, lc = (tid & 15) * 4;
+  uint16_t* x = ns_x(p, g, mi, 0);
   // elements as they lie in memory: 4 columns of rows lr, lr + 16, ..
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -188,30 +186,32 @@ __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
       if (u.zero != nullptr)
         for (int e = 0; e < cnt; ++e) st(u.zero, i + e, 0.f, u.zero_code);
     }
+    if (!g.tall) {
+      st4_pair(x + ns_at(r, g.mp, c), v);
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) tile[lr + 16 * q][lc + e] = v[e];
   }
+  if (!g.tall) return;
   __syncthreads();
-  uint16_t* same = g.tall ? ns_xt(p, g, mi, 0) : ns_x(p, g, mi);   // laid out as in memory
-  uint16_t* turn = g.tall ? ns_x(p, g, mi) : ns_xt(p, g, mi, 0);
-  const int rs = g.tall ? g.np : g.mp, rq = g.tall ? g.mp : g.np;  // their rows
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int a = lr + 16 * q;
-    float v[4], t[4];
+    float t[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = tile[a][lc + e];
-      t[e] = tile[lc + e][a];
-    }
-    st4_pair(same + ns_at(r0 + a, rs, c0 + lc), v);
-    st4_pair(turn + ns_at(c0 + a, rq, r0 + lc), t);
+    for (int e = 0; e < 4; ++e) t[e] = tile[lc + e][a];
+    st4_pair(x + ns_at(c0 + a, g.mp, r0 + lc), t);
   }
 }
 
 // ---- products -----------------------------------------------------------------------------------
 __device__ __forceinline__ NtOperand ns_op(const uint16_t* base, int row0, int rows) {
   return {reinterpret_cast<const char*>(base + (int64_t)row0 * 64), rows - row0, 0, (int64_t)rows * 128};
+}
+// columns col0 .. of a buffer of `rows` x `cols`, as the rows of a turned operand
+__device__ __forceinline__ NtOperand ns_op_turned(const uint16_t* base, int rows, int col0, int cols) {
+  return {reinterpret_cast<const char*>(base + ns_at(0, rows, col0)), cols - col0, 0, (int64_t)rows * 128};
 }
 
 // A 16 x 16 tile turned within the wave: lane l holds rows 4 (l >> 4) .. + 3 of column l & 15, and gets columns
@@ -237,6 +237,7 @@ __device__ __forceinline__ void ns_tri(int t, int nt, int& ti, int& tj) {
 }
 
 // Symmetric m x m products.  kGram: A = X X^T; kPoly: P = a I + b A + c A^2; kMul: L R of two slots.
+// (ls, rs: the operands' slots, of kGram the version of X; ds: the result's)
 enum NsKind { kGram, kPoly, kMul };
 
 template <class C, int KIND>
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int ls, in
   nt_f32x4 acc[C::TA][C::TB];
   const int a0 = tj * C::BA, b0 = ti * C::BB;  // 4 consecutive elements of a lane run along rows of A: columns of C
   if constexpr (KIND == kGram) {
-    const uint16_t* x = ns_x(p, g, mi);
+    const uint16_t* x = ns_x(p, g, mi, ls);
     nt_loop<C>(ring, ns_op(x, a0, g.mp), ns_op(x, b0, g.mp), 0, g.np * 4, acc);
   } else {
     const uint16_t *l = ns_sq(p, g, mi, ls), *r = ns_sq(p, g, mi, rs);
@@ -306,8 +307,9 @@ __global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int ls, in
     }
 }
 
-// X' = Q X.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X'
-// and its transpose (the other version) are stored for the next group of steps.
+// X' = Q X, X read across its lines (TURN), so that it need not be kept both ways: writing X^T beside X took 36 of 52 us
+// at 23 x 256 x 2304.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X' is the
+// other version of X for the next group of steps.
 template <class C, bool FINAL>
 __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int qs, int ver) {
   __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
@@ -318,33 +320,34 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
   id = nt_xcd_item(id, g.count * mt * nt);
   const int mi = id / (mt * nt), t = id % (mt * nt);
   const int m0 = t % mt * C::BA, n0 = t / mt * C::BA;
-  // the operand whose rows are consecutive in the result's memory comes first (4 elements per lane)
-  const bool turned = FINAL && g.tall;
-  const NtOperand q = ns_op(ns_sq(p, g, mi, qs), m0, g.mp);
-  const NtOperand x = ns_op(ns_xt(p, g, mi, ver), n0, g.np);
-  NtOperand A = turned ? q : x, B = turned ? x : q;
   nt_f32x4 acc[C::TA][C::TB];
-  nt_loop<C>(ring, A, B, 0, g.mp * 4, acc);
+  nt_loop<C>(ring, ns_op_turned(ns_x(p, g, mi, ver), g.mp, n0, g.np), ns_op(ns_sq(p, g, mi, qs), m0, g.mp), 0, g.mp * 4,
+             acc);
   const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
-  const int a0 = turned ? m0 : n0, b0 = turned ? n0 : m0;
-  if constexpr (FINAL) {
-    const float f = 1.f / (kNsP * kNsX);
-    const int64_t off = p.off[g.first + mi];
-    const float lr = u.lr != nullptr ? *u.lr : 0.f;
+  const int64_t off = p.off[g.first + mi];
+  const float lr = FINAL && u.lr != nullptr ? *u.lr : 0.f;
+  float* scratch = C::scratch(ring);
+  uint16_t* dx = ns_x(p, g, mi, ver ^ 1);
 #pragma unroll
-    for (int i = 0; i < C::TA; ++i)
+  for (int i = 0; i < C::TA; ++i)
 #pragma unroll
-      for (int j = 0; j < C::TB; ++j) {
-        if (!C::mine(i, j)) continue;
-        const int c = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4;
-        const int r = b0 + (wb * C::TB + j) * 16 + (lane & 15);
+    for (int j = 0; j < C::TB; ++j) {
+      if (!C::mine(i, j)) continue;
+      // the tile's first n and m (wave-uniform); a lane has n0 + 4 (lane >> 4) .. + 3 of m0 + (lane & 15)
+      const int tn = n0 + (wa * C::TA + i) * 16, tm = m0 + (wb * C::TB + j) * 16;
+      if (tn >= g.np || tm >= g.mp) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (FINAL ? 1.f / (kNsP * kNsX) : 1.f / kNsP);
+      if constexpr (!FINAL) {
+        st4_pair(dx + ns_at(tm + (lane & 15), g.mp, tn + (lane >> 4) * 4), v);
+      } else {
+        if (g.tall) ns_turn(scratch, lane, v, v);
+        const int r = (g.tall ? tn : tm) + (lane & 15), c = (g.tall ? tm : tn) + (lane >> 4) * 4;
         if (r >= g.rows || c >= g.cols) continue;
         const int cnt = min(4, g.cols - c);
         const int64_t at = off + (int64_t)r * g.cols + c;
         const bool vec = u.vec && at % 4 == 0 && cnt == 4;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * f;
         if (u.w != nullptr) {
           float w[4];
           ns_ld4(u.w, at, 0, vec, cnt, w);
@@ -361,24 +364,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
           }
         }
       }
-  } else {
-    float* scratch = C::scratch(ring);
-    uint16_t *dx = ns_x(p, g, mi), *dt = ns_xt(p, g, mi, ver ^ 1);
-#pragma unroll
-    for (int i = 0; i < C::TA; ++i)
-#pragma unroll
-      for (int j = 0; j < C::TB; ++j) {
-        if (!C::mine(i, j)) continue;
-        if (b0 + (wb * C::TB + j) * 16 >= g.mp || a0 + (wa * C::TA + i) * 16 >= g.np) continue;  // (wave-uniform)
-        const int ca = a0 + (wa * C::TA + i) * 16, cb = b0 + (wb * C::TB + j) * 16;  // first n, first m of the tile
-        float v[4], t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (1.f / kNsP);
-        ns_turn(scratch, lane, v, t);
-        st4_pair(dx + ns_at(cb + (lane & 15), g.mp, ca + (lane >> 4) * 4), v);
-        st4_pair(dt + ns_at(ca + (lane & 15), g.np, cb + (lane >> 4) * 4), t);
-      }
-  }
+    }
 }
 
 // Tiles and their measured cost: microseconds per K tile with one block per CU alone and with every slot taken, slots
@@ -512,7 +498,7 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
   int ver = 0;
   for (int done = 0; done < steps; ver ^= 1) {
     int q = kP0;
-    ns_sym<kGram>(p, tg, gram, 0, 0, kA, st);
+    ns_sym<kGram>(p, tg, gram, ver, 0, kA, st);
     ns_sym<kPoly>(p, ts, sym, kA, kA, kP0, st);
     if (steps - done >= 2) {
       ns_sym<kMul>(p, ts, sym, kP0, kA, kT, st);
@@ -523,7 +509,7 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     }
     done += q == kQ ? 2 : 1;
     ns_with_tile(tr, [&](auto c) {
-      using C = decltype(c);
+      using C = typename decltype(c)::Turned;
       if (done < steps) ns_apply_kernel<C, false><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
       else ns_apply_kernel<C, true><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
     });

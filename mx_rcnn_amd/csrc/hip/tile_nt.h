@@ -34,6 +34,10 @@ constexpr uint32_t kNtOob = 0x80000000u;  // past any record count (windows are 
 // K tile to the next.  A block's K tile is then one run of memory.  (Row after row, a K tile of fc6's 4096 x 25088
 // touched one line in each of 256 rows 100 KB apart: 3.1 ms for X X^T instead of 1.7.)
 // int8 operands are the caller's rows, `ld` bytes apart (a multiple of 16).
+// TURN: A lies in panels the other way round, lines of k with 32 of A's rows each: panel after panel (`step` bytes) of
+// 32 rows, `rows` a multiple of 32.  A K tile is then 32 lines of each of BA / 32 panels, line k of panel p in LDS row
+// 32 p + k, and a fragment's 8 k values of one row come together in ds_read_b64_tr_b16: of a group of 16 lanes, lane
+// 4 i + j gives the address of elements 4 j .. 4 j + 3 of line i, and lane r receives element r of the four lines.
 struct NtOperand {
   const char* base;
   int rows;  // rows that exist (may exceed the tile)
@@ -43,10 +47,12 @@ struct NtOperand {
 
 // fp16 pairs or int8; BA x BB output tile; KG groups of WA x WB waves, each with every KG-th K tile (joined at the
 // end); NR stages of KG K tiles in the LDS ring; RUN: stages summed apart (0: all); AHEAD: fragments of a stage are
-// read while those of the one before are multiplied.
-template <bool PAIR_, int BA_, int BB_, int KG_, int WA_, int WB_, int NR_, int RUN_ = 0, bool AHEAD_ = false>
+// read while those of the one before are multiplied.  TURN: operand A is read across its lines (NtOperand).
+template <bool PAIR_, int BA_, int BB_, int KG_, int WA_, int WB_, int NR_, int RUN_ = 0, bool AHEAD_ = false,
+          bool TURN_ = false>
 struct NtCfg {
-  static constexpr bool PAIR = PAIR_, AHEAD = AHEAD_;
+  static constexpr bool PAIR = PAIR_, AHEAD = AHEAD_, TURN = TURN_;
+  using Turned = NtCfg<PAIR_, BA_, BB_, KG_, WA_, WB_, NR_, RUN_, AHEAD_, true>;
   static constexpr int BA = BA_, BB = BB_, KG = KG_, WA = WA_, WB = WB_, NR = NR_, RUN = RUN_;
   static constexpr int GROUP = WA * WB, WAVES = KG * GROUP, THREADS = 64 * WAVES;
   static constexpr int TA = BA / WA / 16, TB = BB / WB / 16;
@@ -58,6 +64,7 @@ struct NtCfg {
   static constexpr int JOIN = KG > 1 ? WAVES * TA * TB * 1024 : 0;  // accumulators exchanged between groups
   static constexpr int LDS = RING > JOIN + WAVES * 1280 ? RING : JOIN + WAVES * 1280;
   using Acc = typename std::conditional<PAIR, nt_f32x4, nt_i32x4>::type;
+  static_assert(!TURN || (PAIR && BA % 32 == 0), "turned operands are panels of pairs");
   static_assert(!PAIR || KG * ROWS % (8 * WAVES) == 0, "pairs: every load has its rows");
   static_assert(BA % (16 * WA) == 0 && BB % (16 * WB) == 0, "whole 16x16 tiles per wave");
   static_assert(NR >= 2 && LDS <= 160 * 1024 && (NR - 1) * LPT < 64, "ring depth (vmcnt counts to 63)");
@@ -110,6 +117,30 @@ __device__ __forceinline__ uint4 nt_frag(const char* T, int row, int half, int l
   return *reinterpret_cast<const uint4*>(T + row * 128 + (((half * 4 + (lane >> 4)) ^ ((row >> 1) & 7)) << 4));
 }
 
+// The same of a turned operand, rows row0 .. row0 + 15 of the K tile (row0 a multiple of 16).  Its lines are swizzled by
+// pairs of chunks: the 8 lines that 32 lanes read at once are 4 apart in (k >> 1), in two runs, and take 32 bytes each.
+__device__ __forceinline__ int nt_turn_swizzle(int k) { return ((k >> 1) & 1) << 1 | ((k >> 3) & 1) << 2; }
+typedef short nt_s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ nt_s16x4 nt_turned_read(const char* at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) nt_s16x4*)at);
+}
+__device__ __forceinline__ uint4 nt_turned_frag(const char* T, int row0, int half, int lane) {
+  uint2 v[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int k = 8 * (lane >> 4) + 4 * t + ((lane & 15) >> 2);
+    const int chunk = half * 4 + ((row0 & 16) >> 3) + ((lane & 3) >> 1);
+    v[t] = __builtin_bit_cast(uint2, nt_turned_read(T + ((row0 & ~31) + k) * 128 + ((chunk ^ nt_turn_swizzle(k)) << 4) +
+                                                    (lane & 1) * 8));
+  }
+  return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+}
+template <class C>
+__device__ __forceinline__ uint4 nt_a_frag(const char* T, int row0, int half, int lane) {
+  if constexpr (C::TURN) return nt_turned_frag(T, row0, half, lane);
+  else return nt_frag(T, row0 + (lane & 15), half, lane);
+}
+
 // The products of one row of fragments with all columns.
 template <class C>
 __device__ __forceinline__ void nt_row_mma(const uint4 (&a)[2], const uint4 (&b)[2][C::TB],
@@ -140,7 +171,7 @@ struct NtFrags {
 #pragma unroll
     for (int i = 0; i < C::TA; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) a[i][h] = nt_frag(T, (wa * C::TA + i) * 16 + r16, h, lane);
+      for (int h = 0; h < 2; ++h) a[i][h] = nt_a_frag<C>(T, (wa * C::TA + i) * 16, h, lane);
   }
   __device__ __forceinline__ void mma(typename C::Acc (&acc)[C::TA][C::TB]) const {
 #pragma unroll
@@ -159,12 +190,12 @@ __device__ __forceinline__ void nt_tile_mma(const char* T, int wa, int wb, int l
 #pragma unroll
     for (int j = 0; j < C::TB; ++j) b[h][j] = nt_frag(T, C::BA + (wb * C::TB + j) * 16 + r16, h, lane);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) a[0][h] = nt_frag(T, wa * C::TA * 16 + r16, h, lane);
+  for (int h = 0; h < 2; ++h) a[0][h] = nt_a_frag<C>(T, wa * C::TA * 16, h, lane);
 #pragma unroll
   for (int i = 0; i < C::TA; ++i) {
     if (i + 1 < C::TA) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) a[(i + 1) & 1][h] = nt_frag(T, (wa * C::TA + i + 1) * 16 + r16, h, lane);
+      for (int h = 0; h < 2; ++h) a[(i + 1) & 1][h] = nt_a_frag<C>(T, (wa * C::TA + i + 1) * 16, h, lane);
     }
     __builtin_amdgcn_sched_barrier(0);  // (the compiler would sink these reads behind the products)
     nt_row_mma<C>(a[i & 1], b, acc[i]);
@@ -200,6 +231,10 @@ __device__ __forceinline__ void nt_loop_body(char* lds, const char* __restrict__
     chunk[i] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
     if constexpr (C::PAIR) {
       off[i] = row * 128 + chunk[i];
+      if (C::TURN && !is_b)
+        off[i] = row < arows ? (uint32_t)(row >> 5) * (uint32_t)A.step + (row & 31) * 128 +
+                                   ((lane & 7) ^ nt_turn_swizzle(row & 31)) * 16
+                             : kNtOob;
     } else {
       chunk[i] += g * 128;
       off[i] = g < C::KG && row < (is_b ? brows : arows) ? (uint32_t)row * (is_b ? B.ld : A.ld) + (uint32_t)chunk[i] : kNtOob;
@@ -219,8 +254,9 @@ __device__ __forceinline__ void nt_loop_body(char* lds, const char* __restrict__
         // a window of the operand's rows at this K tile; none past the end
         const int t = kt * C::KG + r0 / C::ROWS;
         const bool in = t * 128 < k_hi;
-        const char* at = is_b ? b_base + t * B.step : a_base + t * A.step;
-        nt_dma(nt_rsrc(at, in ? (is_b ? brows : arows) * 128 : 0), dst, off[i], 0);
+        const char* at = is_b ? b_base + t * B.step : a_base + (C::TURN ? t * 4096 : t * A.step);
+        const int bytes = C::TURN && !is_b ? (arows / 32 - 1) * (int)A.step + 4096 : (is_b ? brows : arows) * 128;
+        nt_dma(nt_rsrc(at, in ? bytes : 0), dst, off[i], 0);
       } else {
         const int k = k_lo + kt * 128 * C::KG;
         nt_dma(is_b ? rb : ra, dst, k + chunk[i] < k_hi ? off[i] : kNtOob, k);
