@@ -307,11 +307,112 @@ __global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int ls, in
     }
 }
 
+// The m x m products of a group of steps in one block, for mp <= kNsChain: A (from kA) to P0, or with `two` to Q = P1 P0,
+// in slot kQ.  Two matrices of LDS, in the layout of a K tile of the products above, K tile after K tile: s0 holds A, then
+// T = P0 A, A' = T P0 and P1; s1 holds P0.  A product's 16 x 16 tiles on and above the diagonal are dealt to the 16
+// waves, held in registers until every wave has read its operands, and written with their mirror images.
+constexpr int kNsChain = 128;
+
+__device__ __forceinline__ int ns_lds_at(int row, int rows, int col) {  // byte of the hi value; the lo value's is ^ 64
+  return ((col >> 5) * rows + row) * 128 + ((((col & 31) >> 3) ^ ((row >> 1) & 7)) << 4) + (col & 7) * 2;
+}
+
+__global__ void __launch_bounds__(1024) ns_chain_kernel(NsArgs p, int two) {
+  constexpr int kTiles = (kNsChain / 16) * (kNsChain / 16 + 1) / 2;
+  constexpr int kMine = (kTiles + 15) / 16;  // tiles of a wave, at most
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kNsChain * kNsChain * 4 + 16 * 1280];
+  char *s0 = lds, *s1 = lds + kNsChain * kNsChain * 4;
+  int mi = blockIdx.x;
+  const int k = ns_find(p, mi, &NsGroup::chain);
+  const NsGroup& g = p.g[k];
+  const int mp = g.mp, nt = mp / 16, tri = nt * (nt + 1) / 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float* scratch = reinterpret_cast<float*>(lds + 2 * kNsChain * kNsChain * 4 + wave * 1280);
+  const char* a = reinterpret_cast<const char*>(ns_sq(p, g, mi, kA));
+  uint16_t* out = ns_sq(p, g, mi, kQ);
+  for (int i = threadIdx.x; i < mp * mp / 4; i += 1024) {  // 16 bytes: chunk i & 7 of line i >> 3
+    const int row = (i >> 3) % mp;
+    *reinterpret_cast<uint4*>(s0 + (i >> 3) * 128 + (((i & 7) ^ ((row >> 1) & 7)) << 4)) =
+        reinterpret_cast<const uint4*>(a)[i];
+  }
+  __syncthreads();
+  // dst = a I + b L + c L L (poly) or L R, to LDS or (nullptr) to `out`
+  const auto product = [&](const char* L, const char* R, char* dst, bool poly) {
+    nt_f32x4 acc[kMine];
+    int ti[kMine], tj[kMine];
+#pragma unroll
+    for (int t = 0; t < kMine; ++t) {
+      acc[t] = nt_f32x4{0, 0, 0, 0};
+      if (wave + 16 * t >= tri) continue;
+      ns_tri(wave + 16 * t, nt, ti[t], tj[t]);
+      for (int kt = 0; kt < mp / 32; ++kt) {
+        uint4 x[2], y[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[h] = nt_frag(L + kt * mp * 128, tj[t] * 16 + (lane & 15), h, lane);
+          y[h] = nt_frag(R + kt * mp * 128, ti[t] * 16 + (lane & 15), h, lane);
+        }
+        acc[t] = nt_mma(x[0], y[1], acc[t]);
+        acc[t] = nt_mma(x[1], y[0], acc[t]);
+        acc[t] = nt_mma(x[0], y[0], acc[t]);
+      }
+    }
+    __syncthreads();
+    const auto put = [&](int row, int col, const float v[4]) {
+      if (dst == nullptr) {
+        st4_pair(out + ns_at(row, mp, col), v);
+        return;
+      }
+      uint16_t h[4], l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split_f16(v[e], h[e], l[e]);
+      const int at = ns_lds_at(row, mp, col);
+      *reinterpret_cast<ushort4*>(dst + at) = make_ushort4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<ushort4*>(dst + (at ^ 64)) = make_ushort4(l[0], l[1], l[2], l[3]);
+    };
+#pragma unroll
+    for (int t = 0; t < kMine; ++t) {
+      if (wave + 16 * t >= tri) continue;
+      const int row = ti[t] * 16 + (lane & 15), col = tj[t] * 16 + (lane >> 4) * 4;
+      float v[4], m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[t][e] * (poly ? 1.f / (kNsX * kNsX) : 1.f / kNsP);
+      if (poly) {
+        const int at = ns_lds_at(row, mp, col);
+        const ushort4 h = *reinterpret_cast<const ushort4*>(L + at), l = *reinterpret_cast<const ushort4*>(L + (at ^ 64));
+        const float av[4] = {f16_to_f32(h.x) + f16_to_f32(l.x), f16_to_f32(h.y) + f16_to_f32(l.y),
+                             f16_to_f32(h.z) + f16_to_f32(l.z), f16_to_f32(h.w) + f16_to_f32(l.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = kNsP * ((col + e == row ? kNsA : 0.f) + kNsB * (av[e] / kNsX) + kNsC * v[e]);
+      }
+      ns_turn(scratch, lane, v, m);
+      if (ti[t] == tj[t]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = col + e >= row ? v[e] : m[e];
+      } else {
+        put(tj[t] * 16 + (lane & 15), ti[t] * 16 + (lane >> 4) * 4, m);
+      }
+      put(row, col, v);
+    }
+    __syncthreads();
+  };
+  if (!two) {
+    product(s0, s0, nullptr, true);
+    return;
+  }
+  product(s0, s0, s1, true);
+  product(s1, s0, s0, false);
+  product(s0, s1, s0, false);
+  product(s0, s0, s0, true);
+  product(s0, s1, nullptr, false);
+}
+
 // X' = Q X, X read across its lines (TURN), so that it need not be kept both ways: writing X^T beside X took 36 of 52 us
 // at 23 x 256 x 2304.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X' is the
 // other version of X for the next group of steps.
 template <class C, bool FINAL>
-__global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int qs, int ver) {
+__global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int ver) {
   __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
   int id = blockIdx.x;
   const int k = ns_find(p, id, &NsGroup::rect);
@@ -321,7 +422,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
   const int mi = id / (mt * nt), t = id % (mt * nt);
   const int m0 = t % mt * C::BA, n0 = t / mt * C::BA;
   nt_f32x4 acc[C::TA][C::TB];
-  nt_loop<C>(ring, ns_op_turned(ns_x(p, g, mi, ver), g.mp, n0, g.np), ns_op(ns_sq(p, g, mi, qs), m0, g.mp), 0, g.mp * 4,
+  nt_loop<C>(ring, ns_op_turned(ns_x(p, g, mi, ver), g.mp, n0, g.np), ns_op(ns_sq(p, g, mi, kQ), m0, g.mp), 0, g.mp * 4,
              acc);
   const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
   const int64_t off = p.off[g.first + mi];
@@ -382,7 +483,7 @@ struct NsTile {
   double alone, full, round;
 };
 constexpr NsTile kNsTiles[4] = {
-    {64, 256, 0.28, 0.30, 6.0}, {128, 512, 0.75, 1.40, 7.0}, {192, 256, 1.31, 1.68, 9.0}, {256, 256, 1.95, 2.45, 12.0}};
+    {64, 256, 0.28, 0.30, 6.0}, {128, 512, 0.75, 1.40, 7.0}, {192, 256, 1.31, 1.68, 9.0}, {256, 256, 1.95, 2.45, 20.0}};
 
 enum NsLaunch { kLaunchGram, kLaunchSym, kLaunchRect };
 
@@ -476,7 +577,7 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     return a.np != b.np ? a.np > b.np : a.mp > b.mp;
   });
   const int tg = ns_pick(p.g, ng, kLaunchGram), ts = ns_pick(p.g, ng, kLaunchSym), tr = ns_pick(p.g, ng, kLaunchRect);
-  int ew = 0, init = 0, gram = 0, sym = 0, rect = 0;
+  int ew = 0, init = 0, gram = 0, sym = 0, rect = 0, chain = 0;
   int64_t wat = 0;
   for (int k = 0; k < ng; ++k) {
     NsGroup& g = p.g[k];
@@ -486,6 +587,8 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     g.gram = gram;
     g.sym = sym;
     g.rect = rect;
+    g.chain = chain;
+    chain += g.count;
     wat += ns_ws_elements(g);
     ew += g.count * g.parts;
     init += g.count * (g.mp / 64) * (g.np / 64);
@@ -495,23 +598,28 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
   }
   ns_norm_kernel<<<ew, 256, 0, st>>>(p, u);
   ns_init_kernel<<<init, 256, 0, st>>>(p, u);
+  // products that fit one block each are chained in it: 5 launches less for two steps
+  const bool chained = std::all_of(p.g, p.g + ng, [](const NsGroup& g) { return g.mp <= kNsChain; });
   int ver = 0;
   for (int done = 0; done < steps; ver ^= 1) {
-    int q = kP0;
+    const bool two = steps - done >= 2;
     ns_sym<kGram>(p, tg, gram, ver, 0, kA, st);
-    ns_sym<kPoly>(p, ts, sym, kA, kA, kP0, st);
-    if (steps - done >= 2) {
-      ns_sym<kMul>(p, ts, sym, kP0, kA, kT, st);
-      ns_sym<kMul>(p, ts, sym, kT, kP0, kA, st);
-      ns_sym<kPoly>(p, ts, sym, kA, kA, kP1, st);
-      ns_sym<kMul>(p, ts, sym, kP1, kP0, kQ, st);
-      q = kQ;
+    if (chained) {
+      ns_chain_kernel<<<chain, 1024, 0, st>>>(p, two);
+    } else {
+      ns_sym<kPoly>(p, ts, sym, kA, kA, two ? kP0 : kQ, st);
+      if (two) {
+        ns_sym<kMul>(p, ts, sym, kP0, kA, kT, st);
+        ns_sym<kMul>(p, ts, sym, kT, kP0, kA, st);
+        ns_sym<kPoly>(p, ts, sym, kA, kA, kP1, st);
+        ns_sym<kMul>(p, ts, sym, kP1, kP0, kQ, st);
+      }
     }
-    done += q == kQ ? 2 : 1;
+    done += two ? 2 : 1;
     ns_with_tile(tr, [&](auto c) {
       using C = typename decltype(c)::Turned;
-      if (done < steps) ns_apply_kernel<C, false><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
-      else ns_apply_kernel<C, true><<<rect, C::THREADS, 0, st>>>(p, u, q, ver);
+      if (done < steps) ns_apply_kernel<C, false><<<rect, C::THREADS, 0, st>>>(p, u, ver);
+      else ns_apply_kernel<C, true><<<rect, C::THREADS, 0, st>>>(p, u, ver);
     });
   }
 }
