@@ -803,56 +803,86 @@ std::vector<Tensor> quantize_rows(const Tensor& x) {
   Tensor s = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
   if (x.size(0) > 0)
     mxr::quantize_rows(x.data_ptr(), code, x.size(0), x.stride(0), (int)x.size(1), q.data_ptr<int8_t>(),
-                       s.data_ptr<float>(), cur_stream());
+                       (int)x.size(1), s.data_ptr<float>(), cur_stream());
   LAUNCH_CHECK("quantize_rows");
   return {q, s};
 }
 
-Tensor int8_matmul(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, c10::optional<Tensor> bias,
-                   bool relu, int64_t code) {
+static void check_row_vec(const Tensor& t, int64_t n, const Tensor& x, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous() &&
+                  t.device() == x.device(),
+              "int8_matmul: ", what, " must be contiguous fp32 (", n, ",) on the operands' device");
+}
+
+// The product's arguments from its tensors, but for xs and the output: x is (M, K), of int8 rows or of those to quantize.
+static mxr::Int8Args int8_args(const Tensor& x, const Tensor& w, const Tensor& ws, const c10::optional<Tensor>& bias,
+                               bool relu, int64_t code) {
   CHECK_DEV(x); CHECK_DEV(w);
-  for (auto* t : {&x, &w})
-    TORCH_CHECK(t->scalar_type() == at::kChar && t->dim() == 2 && (t->stride(1) == 1 || t->size(1) <= 1),
-                "int8_matmul: operands are int8 (rows, K) with K contiguous");
+  TORCH_CHECK(w.scalar_type() == at::kChar && w.dim() == 2 && (w.stride(1) == 1 || w.size(1) <= 1),
+              "int8_matmul: the weight is int8 (N, K) with K contiguous");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   TORCH_CHECK(w.size(1) == K, "int8_matmul: K differs: ", K, " and ", w.size(1));
   TORCH_CHECK(K <= 131071, "int8_matmul: K = ", K, " (int32 sums are exact up to 131071)");
   TORCH_CHECK(M <= (1 << 24) && N <= (1 << 24), "int8_matmul: more than 2^24 rows");
-  const auto vec = [&](const Tensor& t, int64_t n, const char* what) {
-    TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous() &&
-                    t.device() == x.device(),
-                "int8_matmul: ", what, " must be contiguous fp32 (", n, ",) on the operands' device");
-  };
-  vec(xs, M, "xs");
-  vec(ws, N, "ws");
   TORCH_CHECK(w.device() == x.device(), "int8_matmul: operands on different devices");
+  TORCH_CHECK(code >= 0 && code <= 2, "int8_matmul: output type");
+  check_row_vec(ws, N, x, "ws");
   mxr::Int8Args a = {};
   if (bias.has_value() && bias->defined()) {
-    vec(*bias, N, "bias");
+    check_row_vec(*bias, N, x, "bias");
     a.bias = bias->data_ptr<float>();
   }
-  TORCH_CHECK(code >= 0 && code <= 2, "int8_matmul: output type");
-  DevGuard g(x.device());
-  Tensor y = at::empty({M, N}, x.options().dtype(code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf));
-  if (M == 0 || N == 0) return y;
-  a.x = x.data_ptr<int8_t>();
   a.w = w.data_ptr<int8_t>();
-  a.ldx = x.stride(0);
   a.ldw = w.stride(0);
-  a.xs = xs.data_ptr<float>();
   a.ws = ws.data_ptr<float>();
-  a.y = y.data_ptr();
   a.M = M;
   a.N = (int)N;
   a.K = (int)K;
   a.code = (int)code;
   a.relu = relu;
+  return a;
+}
+
+static Tensor int8_run(mxr::Int8Args& a, const at::TensorOptions& o) {
+  Tensor y = at::empty({a.M, a.N}, o.dtype(a.code == 0 ? at::kFloat : a.code == 1 ? at::kBFloat16 : at::kHalf));
+  if (a.M == 0 || a.N == 0) return y;
+  a.y = y.data_ptr();
   const int64_t bytes = mxr::int8_matmul_ws(a);
   Tensor ws_buf;
-  if (bytes > 0) ws_buf = at::empty({bytes}, x.options().dtype(at::kByte));
+  if (bytes > 0) ws_buf = at::empty({bytes}, o.dtype(at::kByte));
   mxr::int8_matmul(a, bytes > 0 ? ws_buf.data_ptr() : nullptr, cur_stream());
   LAUNCH_CHECK("int8_matmul");
   return y;
+}
+
+Tensor int8_matmul(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, c10::optional<Tensor> bias,
+                   bool relu, int64_t code) {
+  TORCH_CHECK(x.scalar_type() == at::kChar && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1),
+              "int8_matmul: x is int8 (M, K) with K contiguous");
+  mxr::Int8Args a = int8_args(x, w, ws, bias, relu, code);
+  check_row_vec(xs, a.M, x, "xs");
+  DevGuard g(x.device());
+  a.x = x.data_ptr<int8_t>();
+  a.ldx = x.stride(0);
+  a.xs = xs.data_ptr<float>();
+  return int8_run(a, x.options());
+}
+
+// quantize_rows and int8_matmul in one call; the rows are laid out for the product (padded to 16 bytes)
+Tensor int8_linear(const Tensor& x, const Tensor& w, const Tensor& ws, c10::optional<Tensor> bias, bool relu) {
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "int8_linear: (M, K) with K contiguous");
+  const int code = ns_code(x, "int8_linear");
+  mxr::Int8Args a = int8_args(x, w, ws, bias, relu, code);
+  DevGuard g(x.device());
+  a.ldx = (a.K + 15) / 16 * 16;
+  a.x_padded = 1;
+  Tensor q = at::empty({a.M * (a.ldx + 4)}, x.options().dtype(at::kChar));  // the rows, then their scales
+  int8_t* rows = q.data_ptr<int8_t>();
+  float* scale = reinterpret_cast<float*>(rows + a.M * a.ldx);
+  a.x = rows;
+  a.xs = scale;
+  if (a.M > 0) mxr::quantize_rows(x.data_ptr(), code, a.M, x.stride(0), a.K, rows, (int)a.ldx, scale, cur_stream());
+  return int8_run(a, x.options());
 }
 
 // ---- BN + ReLU -------------------------------------------------------------------------
@@ -2603,6 +2633,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("momentum"), py::arg("wd"), py::arg("rescale"), py::arg("clip"), py::arg("nesterov"), py::arg("steps"),
         py::arg("eps"), py::arg("w_bf16"), py::arg("planes"), py::arg("zero"), py::arg("plane_stride"));
   m.def("quantize_rows", &quantize_rows, py::arg("x"));
+  m.def("int8_linear", &int8_linear, py::arg("x"), py::arg("w"), py::arg("ws"), py::arg("bias"), py::arg("relu"));
   m.def("int8_matmul", &int8_matmul, py::arg("x"), py::arg("xs"), py::arg("w"), py::arg("ws"), py::arg("bias"),
         py::arg("relu"), py::arg("code"));
   m.def("head_bwd", &head_bwd, py::arg("x"), py::arg("dys"), py::arg("ws"), py::arg("dws"), py::arg("dw_acc"),

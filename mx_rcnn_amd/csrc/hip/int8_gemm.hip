@@ -69,16 +69,16 @@ __device__ __forceinline__ uint2 to_i8x8(const Raw8<CODE>& v, float s, float inv
 // T threads per row (a wave: four rows per block), which hold it in registers while its peak is found -- NV times eight
 // values each -- so that x is read once; HELD = false: a row longer than that is read twice, the second time from the
 // caches.  Rows have at least eight values: a thread whose eight would pass the end takes the last eight, and writes
-// what its neighbour writes.
+// what its neighbour writes.  Rows of q are ldq apart, with zeros behind K.
 template <int CODE, int T, int NV, bool HELD>
 __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void* __restrict__ x, int64_t ld_, int64_t rows,
-                                                                     int K, int8_t* __restrict__ q,
+                                                                     int K, int8_t* __restrict__ q, int ldq,
                                                                      float* __restrict__ scale) {
   const int tid = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * (T < 256 ? 256 / T : 1) + threadIdx.x / T;
   if (row >= rows) return;  // (whole waves: rows share a block only where a row is a wave)
   const int64_t x0 = row * ld_;
-  int8_t* out = q + row * K;
+  int8_t* out = q + row * ldq;
   Raw8<CODE> v[HELD ? NV : 1];
   uint32_t peak = 0;
   if constexpr (HELD) {
@@ -107,7 +107,10 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void*
   const float s = row_scale(peak);
   const bool bad = s != s;
   const float inv = 1.f / s;
-  if (tid == 0) scale[row] = s;
+  if (tid == 0) {
+    scale[row] = s;
+    for (int k = K; k < ldq; ++k) out[k] = 0;
+  }
   const auto put = [&](const Raw8<CODE>& d, int k) {
     const uint2 w = bad ? make_uint2(0, 0) : to_i8x8(d, s, inv);
     __builtin_memcpy(out + min(k, K - 8), &w, 8);
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void*
 
 // Rows of fewer than eight values: a thread each.
 __global__ void __launch_bounds__(256) quantize_short_kernel(const void* __restrict__ x, int code, int64_t ld_,
-                                                             int64_t rows, int K, int8_t* __restrict__ q,
+                                                             int64_t rows, int K, int8_t* __restrict__ q, int ldq,
                                                              float* __restrict__ scale) {
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row >= rows) return;
@@ -134,16 +137,16 @@ __global__ void __launch_bounds__(256) quantize_short_kernel(const void* __restr
   for (int k = 0; k < K; ++k) peak = max(peak, abs_bits(ld(x, row * ld_ + k, code)));
   const float s = row_scale(peak);
   scale[row] = s;
-  for (int k = 0; k < K; ++k) q[row * K + k] = s != s ? 0 : (int8_t)rintf(ld(x, row * ld_ + k, code) / s);
+  for (int k = 0; k < ldq; ++k) q[row * ldq + k] = k >= K || s != s ? 0 : (int8_t)rintf(ld(x, row * ld_ + k, code) / s);
 }
 
 template <int CODE>
-void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, float* scale, hipStream_t st) {
+void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, int ldq, float* scale, hipStream_t st) {
   const auto go = [&](auto kernel, int t) {
     const int per = t < 256 ? 256 / t : 1;
-    kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, scale);
+    kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, ldq, scale);
   };
-  if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, scale);
+  if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, ldq, scale);
   // 2400 x 25088 bf16 with 256 / 512 / 1024 threads per row: 36 / 33 / 41 us (512: 5.5 TB/s)
   else if (K <= 512) go(quantize_kernel<CODE, 64, 1, true>, 64);
   else if (K <= 2048 && rows >= 2048) go(quantize_kernel<CODE, 64, 4, true>, 64);
@@ -168,10 +171,11 @@ __device__ __forceinline__ uint4 load16_tail(const int8_t* row, int k, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Both operands' rows to 16-byte-aligned copies, `lda` bytes apart, zeros behind K: those of w follow those of x.
-__global__ void __launch_bounds__(256) pack_rows_kernel(Int8Args p, int8_t* __restrict__ y, int lda) {
+// Rows of x (the first `mx` blocks) and of w to 16-byte-aligned copies, `lda` bytes apart, zeros behind K, one behind
+// the other.
+__global__ void __launch_bounds__(256) pack_rows_kernel(Int8Args p, int64_t mx, int8_t* __restrict__ y, int lda) {
   const int64_t row = blockIdx.x;
-  const int8_t* src = row < p.M ? p.x + row * p.ldx : p.w + (row - p.M) * p.ldw;
+  const int8_t* src = row < mx ? p.x + row * p.ldx : p.w + (row - mx) * p.ldw;
   for (int k = threadIdx.x * 16; k < lda; k += 4096)
     *reinterpret_cast<uint4*>(y + row * lda + k) = load16_tail(src, k, p.K);
 }
@@ -209,60 +213,101 @@ __device__ __forceinline__ void int8_store(const Int8Args& p, int32_t* part, int
 
 // Few rows of x, or little of everything: each of KG waves reads both operands' fragments of every KG-th K tile
 // straight into registers, two K tiles ahead, with no barrier until the sums of the waves are added up in LDS.  A
-// block has 16 rows of w and 16 TB rows of x, and does without a copy of unaligned rows.  One row against 4096 x 25088:
-// 19.5 us, 5.3 TB/s.
+// block has 16 rows of w and 16 TB rows of x.  One row against 4096 x 25088: 19.5 us, 5.3 TB/s.
+//
+// Rows at any address (ALIGNED = false) need no copy: the 4 or 5 dwords that hold a lane's 16 bytes are loaded and moved
+// down when they are used.  (As one unaligned load they take 5 times as long as an aligned one.)  Behind K the bytes of x
+// are cleared; those of w then do not matter.  The last, partial step over K is read by single dwords, so that what is
+// past the last row's last dword, and only that, is out of the window.
 template <int TB, bool ALIGNED>
 struct Int8Stream {
-  static constexpr int KG = 8, U = 2;
+  static constexpr int KG = 8, U = 2, STEP = U * KG * 128;
   const Int8Args& p;
   int n0, k_hi, r, ch, kg;
   int64_t m0;
   __amdgpu_buffer_rsrc_t rw, rx;
-  uint32_t ow, ox[TB];
+  uint32_t ow, ox[TB];  // of this lane's first byte; unaligned: of its dword
+  int sw, sx[TB];       // unaligned: the byte within the dword
 
   __device__ __forceinline__ Int8Stream(const Int8Args& a, int n, int64_t m, int k)
       : p(a), n0(n), k_hi(k), r(threadIdx.x & 15), ch((threadIdx.x & 63) >> 4 << 4),
         kg(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m) {
     const int wr = min(p.N - n0, 16), xr = (int)min(p.M - m0, (int64_t)16 * TB);
-    const int ldw = (int)p.ldw, ldx = (int)p.ldx;  // (used where rows are aligned: below 2^22)
-    rw = nt_rsrc(reinterpret_cast<const char*>(p.w) + n0 * p.ldw, (wr - 1) * ldw + k_hi);
-    rx = nt_rsrc(reinterpret_cast<const char*>(p.x) + m0 * p.ldx, (xr - 1) * ldx + k_hi);
-    ow = r < wr ? (uint32_t)(r * ldw + ch) : kNtOob;
+    const int ldw = (int)p.ldw, ldx = (int)p.ldx;  // (below 2^22)
+    const char* w = reinterpret_cast<const char*>(p.w) + n0 * p.ldw;
+    const char* x = reinterpret_cast<const char*>(p.x) + m0 * p.ldx;
+    const int w0 = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(w) & 3);
+    const int x0 = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(x) & 3);
+    rw = nt_rsrc(w - w0, (w0 + (wr - 1) * ldw + k_hi + 3) & ~3);
+    rx = nt_rsrc(x - x0, (x0 + (xr - 1) * ldx + k_hi + 3) & ~3);
+    const auto place = [](bool in, int at, uint32_t& off, int& by) {
+      by = at & 3;
+      off = in ? (uint32_t)(at & ~3) : kNtOob;
+    };
+    place(r < wr, w0 + r * ldw + ch, ow, sw);
 #pragma unroll
-    for (int j = 0; j < TB; ++j) ox[j] = j * 16 + r < xr ? (uint32_t)((j * 16 + r) * ldx + ch) : kNtOob;
+    for (int j = 0; j < TB; ++j) place(j * 16 + r < xr, x0 + (j * 16 + r) * ldx + ch, ox[j], sx[j]);
   }
-  struct Frags {
-    uint4 w[U][2], x[U][2][TB];
+  struct Piece {
+    uint4 v;
+    uint32_t next;  // unaligned: the dword behind them
   };
-  __device__ __forceinline__ uint4 row16(const int8_t* base, int64_t ld_, int64_t row, int64_t rows, int k) const {
-    if (row >= rows || k >= k_hi) return make_uint4(0, 0, 0, 0);
-    return load16_tail(base + row * ld_, k, k_hi);
+  struct Frags {
+    Piece w[U][2], x[U][2][TB];
+  };
+  __device__ __forceinline__ int column(int k0, int u, int h) const { return k0 + (u * KG + kg) * 128 + h * 64; }
+  template <bool TAIL>
+  __device__ __forceinline__ void piece(Piece& d, __amdgpu_buffer_rsrc_t rs, uint32_t off, int k) const {
+    if constexpr (ALIGNED) {
+      d.v = nt_load(rs, k + ch < k_hi ? off : kNtOob, k);
+    } else if constexpr (!TAIL) {
+      d.v = nt_load(rs, off, k);
+      d.next = nt_load1(rs, off + 16, k);
+    } else {
+      const uint32_t at = k + ch < k_hi ? off : kNtOob;
+      d.v.x = nt_load1(rs, at, k);
+      d.v.y = nt_load1(rs, at + 4, k);
+      d.v.z = nt_load1(rs, at + 8, k);
+      d.v.w = nt_load1(rs, at + 12, k);
+      d.next = nt_load1(rs, at + 16, k);
+    }
   }
-  __device__ __forceinline__ void load(Frags& d, int k0) const {
+  // the step at k0; `in` (unaligned whole steps): it is not past the last one
+  template <bool TAIL>
+  __device__ __forceinline__ void load(Frags& d, int k0, bool in = true) const {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + (u * KG + kg) * 128 + h * 64;
-        if constexpr (ALIGNED) {
-          const bool in = k + ch < k_hi;
-          d.w[u][h] = nt_load(rw, in ? ow : kNtOob, k);
+        piece<TAIL>(d.w[u][h], rw, in ? ow : kNtOob, k);
 #pragma unroll
-          for (int j = 0; j < TB; ++j) d.x[u][h][j] = nt_load(rx, in ? ox[j] : kNtOob, k);
-        } else {
-          d.w[u][h] = row16(p.w, p.ldw, n0 + r, p.N, k + ch);
-#pragma unroll
-          for (int j = 0; j < TB; ++j) d.x[u][h][j] = row16(p.x, p.ldx, m0 + j * 16 + r, p.M, k + ch);
-        }
+        for (int j = 0; j < TB; ++j) piece<TAIL>(d.x[u][h][j], rx, in ? ox[j] : kNtOob, k);
       }
   }
-  static __device__ __forceinline__ void mma(const Frags& d, nt_i32x4 (&acc)[TB]) {
+  static __device__ __forceinline__ uint4 bytes(const Piece& d, int by) {
+    if constexpr (ALIGNED) return d.v;
+    return make_uint4(__builtin_amdgcn_alignbyte(d.v.y, d.v.x, by), __builtin_amdgcn_alignbyte(d.v.z, d.v.y, by),
+                      __builtin_amdgcn_alignbyte(d.v.w, d.v.z, by), __builtin_amdgcn_alignbyte(d.next, d.v.w, by));
+  }
+  static __device__ __forceinline__ uint32_t keep(uint32_t v, int n) {  // its first n bytes
+    return n >= 4 ? v : n <= 0 ? 0 : v & ((1u << (8 * n)) - 1);
+  }
+  template <bool TAIL>
+  __device__ __forceinline__ void mma(const Frags& d, int k0, nt_i32x4 (&acc)[TB]) const {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w = bytes(d.w[u][h], sw);
+        const int n = k_hi - (k0 + (u * KG + kg) * 128 + h * 64 + ch);  // this lane's bytes up to the end
 #pragma unroll
-        for (int j = 0; j < TB; ++j) acc[j] = nt_mma(d.w[u][h], d.x[u][h][j], acc[j]);
+        for (int j = 0; j < TB; ++j) {
+          uint4 x = bytes(d.x[u][h][j], sx[j]);
+          if (!ALIGNED && TAIL) x = make_uint4(keep(x.x, n), keep(x.y, n - 4), keep(x.z, n - 8), keep(x.w, n - 12));
+          acc[j] = nt_mma(w, x, acc[j]);
+        }
+      }
   }
 };
 
@@ -272,18 +317,22 @@ __global__ void __launch_bounds__(512) int8_stream_kernel(Int8Args p, int nt, in
   __shared__ nt_i32x4 sums[S::KG][TB][64];
   const int id = nt_xcd_item(blockIdx.x, nt * mt), lane = threadIdx.x & 63;
   const S s(p, id / mt * 16, (int64_t)(id % mt) * 16 * TB, p.K);
-  constexpr int STEP = S::U * S::KG * 128;
+  constexpr int STEP = S::STEP;
   nt_i32x4 acc[TB];
 #pragma unroll
   for (int j = 0; j < TB; ++j) acc[j] = nt_i32x4{0, 0, 0, 0};
-  typename S::Frags f[2];
-  s.load(f[0], 0);
-  for (int k = 0; k < p.K; k += 2 * STEP) {  // (K tiles past the end are zeros)
-    s.load(f[1], k + STEP);
-    S::mma(f[0], acc);
-    s.load(f[0], k + 2 * STEP);
-    S::mma(f[1], acc);
+  // whole steps (aligned: all; what is past the end is zeros), and an unaligned rest
+  const int end = ALIGNED ? p.K : p.K / STEP * STEP;
+  typename S::Frags f[2], rest;
+  if constexpr (!ALIGNED) s.template load<true>(rest, end);
+  s.template load<false>(f[0], 0, ALIGNED || 0 < end);
+  for (int k = 0; k < end; k += 2 * STEP) {
+    s.template load<false>(f[1], k + STEP, ALIGNED || k + STEP < end);
+    s.template mma<false>(f[0], k, acc);
+    s.template load<false>(f[0], k + 2 * STEP, ALIGNED || k + 2 * STEP < end);
+    s.template mma<false>(f[1], k + STEP, acc);
   }
+  if constexpr (!ALIGNED) s.template mma<true>(rest, end, acc);
 #pragma unroll
   for (int j = 0; j < TB; ++j) sums[s.kg][j][lane] = acc[j];
   __syncthreads();
@@ -368,22 +417,26 @@ struct Int8Plan {
   double us;
 };
 
-bool int8_aligned(const void* q, int64_t ld) {
-  // 16-byte loads, and 32-bit offsets within a tile's rows
-  return (reinterpret_cast<uintptr_t>(q) | (uint64_t)ld) % 16 == 0 && ld < (1 << 22);
+constexpr int64_t kInt8Ld = 1 << 22;  // rows closer than that: 32-bit offsets within a tile's rows
+bool int8_aligned(const void* q, int64_t ld) {  // 16-byte loads
+  return (reinterpret_cast<uintptr_t>(q) | (uint64_t)ld) % 16 == 0 && ld < kInt8Ld;
 }
+bool int8_x_aligned(const Int8Args& a) { return (a.K % 16 == 0 || a.x_padded) && int8_aligned(a.x, a.ldx); }
+bool int8_w_aligned(const Int8Args& a) { return a.K % 16 == 0 && int8_aligned(a.w, a.ldw); }
 
 Int8Plan int8_plan(const Int8Args& a) {
   Int8Plan best = {};
   best.us = 1e30;
-  const bool aligned = a.K % 16 == 0 && int8_aligned(a.x, a.ldx) && int8_aligned(a.w, a.ldw);
+  const bool ax = int8_x_aligned(a), aw = int8_w_aligned(a), aligned = ax && aw;
   const int lda = (a.K + 15) / 16 * 16, nk = std::max(1, div_up(lda, 128));
   const double mn = (double)a.M * a.N, k = a.K;
   const double hbm = ((double)a.N + a.M) * k / 5.2e6;
-  const double pack_us = aligned ? 0 : 4 + 2 * (a.M + a.N) * k / 3e6;
-  const int64_t pack_bytes = aligned ? 0 : ((a.M + a.N) * lda + 255) / 256 * 256;
+  const int64_t packed = (ax ? 0 : a.M) + (aw ? 0 : a.N);  // rows to copy
+  const double pack_us = packed ? 3 + 2 * packed * k / 5e6 : 0;
+  const int64_t pack_bytes = (packed * lda + 255) / 256 * 256;
   for (int s = 0; s < 4; ++s) {  // 16 or 32 rows of x; unaligned rows as they are, or copied first
     if (s >= 2 && aligned) break;
+    if (s < 2 && (a.ldw >= kInt8Ld || a.ldx >= kInt8Ld)) continue;
     Int8Plan p = {};
     p.kind = s & 1;
     p.pack = s >= 2;
@@ -392,7 +445,7 @@ Int8Plan int8_plan(const Int8Args& a) {
     p.mt = div_up(a.M, 16 << p.kind);
     p.splits = 1;
     const double blocks = (double)p.nt * p.mt, rows = std::min<double>(a.M, 16 << p.kind);
-    p.us = std::max(hbm, std::ceil(blocks / 512) * (std::ceil(nk / 16.0) * (aligned || p.pack ? 0.9 : 4.5) + 2)) +
+    p.us = std::max(hbm, std::ceil(blocks / 512) * (std::ceil(nk / 16.0) * (aligned || p.pack ? 0.9 : 1.3) + 2)) +
            blocks * (rows + (p.mt > 1 ? 16 : 0)) * k / 12e6 + 2;
     if (p.pack) {
       p.us += pack_us;
@@ -435,10 +488,11 @@ void int8_tiles(const Int8Args& a, const Int8Plan& p, int32_t* part, hipStream_t
 
 }  // namespace
 
-void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, float* scale, hipStream_t st) {
-  if (code == 0) quantize<0>(x, rows, ld, K, q, scale, st);
-  else if (code == 1) quantize<1>(x, rows, ld, K, q, scale, st);
-  else quantize<2>(x, rows, ld, K, q, scale, st);
+void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, int ldq, float* scale,
+                   hipStream_t st) {
+  if (code == 0) quantize<0>(x, rows, ld, K, q, ldq, scale, st);
+  else if (code == 1) quantize<1>(x, rows, ld, K, q, ldq, scale, st);
+  else quantize<2>(x, rows, ld, K, q, ldq, scale, st);
 }
 
 int64_t int8_matmul_ws(const Int8Args& a) { return int8_plan(a).bytes; }
@@ -448,13 +502,20 @@ void int8_matmul(const Int8Args& args, void* ws, hipStream_t st) {
   const Int8Plan p = int8_plan(a);
   if (p.pack) {
     int8_t* xb = static_cast<int8_t*>(ws);
-    pack_rows_kernel<<<(unsigned)(a.M + a.N), 256, 0, st>>>(a, xb, p.lda);
-    a.x = xb;
-    a.w = xb + a.M * p.lda;
-    a.ldx = a.ldw = a.K = p.lda;
+    const int64_t mx = int8_x_aligned(a) ? 0 : a.M, nw = int8_w_aligned(a) ? 0 : a.N;
+    pack_rows_kernel<<<(unsigned)(mx + nw), 256, 0, st>>>(a, mx, xb, p.lda);
+    if (mx > 0) {
+      a.x = xb;
+      a.ldx = p.lda;
+    }
+    if (nw > 0) {
+      a.w = xb + mx * p.lda;
+      a.ldw = p.lda;
+    }
+    a.K = p.lda;
   }
   if (p.kind < 2) {
-    const bool aligned = a.K % 16 == 0 && int8_aligned(a.x, a.ldx) && int8_aligned(a.w, a.ldw);
+    const bool aligned = int8_x_aligned(a) && int8_w_aligned(a);
     const unsigned grid = (unsigned)(p.nt * p.mt);
     if (p.kind == 0 && aligned) int8_stream_kernel<1, true><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
     else if (p.kind == 0) int8_stream_kernel<1, false><<<grid, 512, 0, st>>>(a, p.nt, p.mt);

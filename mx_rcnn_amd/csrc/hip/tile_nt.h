@@ -102,6 +102,9 @@ typedef uint32_t nt_u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 nt_load(__amdgpu_buffer_rsrc_t rs, uint32_t voff, int soff) {
   return __builtin_bit_cast(uint4, (nt_u32x4)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)voff, soff, 0));
 }
+__device__ __forceinline__ uint32_t nt_load1(__amdgpu_buffer_rsrc_t rs, uint32_t voff, int soff) {  // 4 bytes
+  return __builtin_amdgcn_raw_buffer_load_b32(rs, (int)voff, soff, 0);
+}
 
 __device__ __forceinline__ nt_f32x4 nt_mma(const uint4& a, const uint4& b, nt_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(nt_f16x8, a), __builtin_bit_cast(nt_f16x8, b), c, 0,

@@ -49,7 +49,8 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
             double* part, hipStream_t st);
 
 // ---- 8-bit rows and products (int8_gemm.hip) -----------------------------------------------------
-void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, float* scale,
+// rows of q are ldq >= K bytes apart, zeros behind K
+void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, int ldq, float* scale,
                    hipStream_t st);
 
 struct Int8Args {
@@ -59,6 +60,7 @@ struct Int8Args {
   void* y;  // (M, N) contiguous, storage code 0 / 1 / 2
   int64_t M;
   int N, K, code, relu;
+  int x_padded;  // rows of x hold zeros from K to the next multiple of 16
 };
 int64_t int8_matmul_ws(const Int8Args& a);  // bytes of workspace
 void int8_matmul(const Int8Args& a, void* ws, hipStream_t st);

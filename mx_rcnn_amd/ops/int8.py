@@ -47,8 +47,8 @@ def _rows(t):
 def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16):
     """``relu(xs[:, None] * ws * (xq @ wq.T) + bias)`` of int8 ``xq`` (M, K) and ``wq`` (N, K) with fp32
     scales ``xs`` (M,) and ``ws`` (N,) and fp32 ``bias`` (N,): the sum exact in int32 (K <= 131071), the
-    rest in fp32, rounded once to ``out_dtype`` (fp32, bf16 or fp16).  Rows may lie any stride apart;
-    K, strides and addresses that are multiples of 16 bytes are read in place, others through a copy."""
+    rest in fp32, rounded once to ``out_dtype`` (fp32, bf16 or fp16).  Rows may lie any stride apart, at any
+    address; where there are many of them, those whose K, stride or address is no multiple of 16 are copied first."""
     if out_dtype not in OUT_CODES:
         raise TypeError('int8_matmul: out_dtype fp32, bf16 or fp16, not %s' % (out_dtype,))
     if xq.dim() == 2 and xq.shape[1] > MAX_K:
@@ -78,5 +78,9 @@ def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16)
 def int8_linear(x, wq, ws, bias=None, relu=False):
     """A fully connected layer on floating rows ``x`` (M, K) with an 8-bit weight (``quantize_rows`` of the
     (N, K) weight): the rows quantized, multiplied, scaled back; result in x's type."""
-    xq, xs = quantize_rows(x)
+    if x.is_cuda:  # one call; the rows are quantized into the layout that the product reads
+        if x.dim() == 2 and x.shape[1] > MAX_K:
+            raise ValueError('int8_linear: K = %d (int32 sums are exact up to %d)' % (x.shape[1], MAX_K))
+        return need_ext().int8_linear(_rows(x.detach()), _rows(wq), ws, bias, relu)
+    xq, xs = quantize_rows(x.detach())
     return int8_matmul(xq, xs, wq, ws, bias, relu, x.dtype)

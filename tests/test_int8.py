@@ -153,6 +153,34 @@ def test_int8_matmul_strides(dev, M, N, K):
         _check_product(y, (xq, xs, wq, ws), None, False, torch.float32)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('M,N', [(5, 20), (33, 17), (70, 130)])
+def test_int8_matmul_any_address(cuda, M, N):
+    """Rows that start at every byte of a dword and end at every place of a load: with scales of 1 and an fp32
+    result, the sum rounded once.  What lies between and behind the rows is not zero."""
+    gen = torch.Generator().manual_seed(3)
+    one = torch.ones(max(M, N), device=cuda)
+    for K in (1, 3, 15, 16, 17, 63, 64, 65, 79, 127, 129, 2047, 2048, 2049, 2064, 4111, 6200):
+        for at, gap in ((0, 0), (1, 0), (2, 3), (3, 5), (0, 1), (4, 4)):
+            flat = [torch.randint(-128, 128, (at + r * (K + gap),), generator=gen).to(torch.int8) for r in (M, N)]
+            x, w = (torch.as_strided(f.to(cuda), (r, K), (K + gap, 1), at) for f, r in zip(flat, (M, N)))
+            got = ops.int8_matmul(x, one[:M], w, one[:N], out_dtype=torch.float32)
+            want = (x.cpu().to(torch.int64) @ w.cpu().to(torch.int64).t()).float()
+            assert torch.equal(got.cpu(), want), (K, at, gap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_int8_linear_is_its_two_parts(cuda, dtype):
+    gen = torch.Generator().manual_seed(4)
+    for M, N, K in ((1, 9, 1), (1, 40, 7), (3, 8, 17), (20, 300, 1001), (300, 96, 515), (130, 257, 4096), (2, 5, 33000)):
+        x = torch.randn(M, K, generator=gen).to(dtype).to(cuda)
+        wq, ws = ops.quantize_rows(torch.randn(N, K, generator=gen).to(cuda))
+        b = torch.randn(N, generator=gen).to(cuda)
+        want = ops.int8_matmul(*ops.quantize_rows(x), wq, ws, b, relu=True, out_dtype=dtype)
+        assert torch.equal(ops.int8_linear(x, wq, ws, b, relu=True), want), (M, N, K)
+
+
 @on_both
 def test_int8_matmul_extremes(dev):
     """The largest sums (K = 131071, all -128), single steps, and a NaN scale that stays in its row."""
