@@ -307,6 +307,71 @@ __global__ void __launch_bounds__(C::THREADS) ns_sym_kernel(NsArgs p, int ls, in
     }
 }
 
+// A = X X^T of few matrices with long rows: a tile's K is cut into g.splits runs of g.run_k K tiles, whose fp32 sums
+// go to the version of X that is not in use (splits <= np / mp), row-major mp x mp each; ns_join_kernel adds them up.
+template <class C>
+__global__ void __launch_bounds__(C::THREADS) ns_gram_part_kernel(NsArgs p, int ver) {
+  __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
+  int id = blockIdx.x;
+  const int k = ns_find(p, id, &NsGroup::gram);
+  const NsGroup& g = p.g[k];
+  const int nt = (g.mp + C::BA - 1) / C::BA, tri = nt * (nt + 1) / 2;
+  id = nt_xcd_item(id, g.count * tri * g.splits);
+  const int mi = id / (tri * g.splits), sp = id / tri % g.splits;
+  int ti, tj;
+  ns_tri(id % tri, nt, ti, tj);
+  const int a0 = tj * C::BA, b0 = ti * C::BB, k0 = sp * g.run_k;
+  const uint16_t* x = ns_x(p, g, mi, ver) + (int64_t)k0 * g.mp * 64;
+  nt_f32x4 acc[C::TA][C::TB];
+  nt_loop<C>(ring, ns_op(x, a0, g.mp), ns_op(x, b0, g.mp), 0, min(g.run_k, g.np / 32 - k0) * 128, acc);
+  float* dst = reinterpret_cast<float*>(ns_x(p, g, mi, ver ^ 1)) + (int64_t)sp * g.mp * g.mp;
+  const int lane = threadIdx.x & 63, wa = C::wa(), wb = C::wb();
+#pragma unroll
+  for (int i = 0; i < C::TA; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TB; ++j) {
+      if (!C::mine(i, j)) continue;
+      const int ca = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4, cb = b0 + (wb * C::TB + j) * 16 + (lane & 15);
+      *reinterpret_cast<nt_f32x4*>(dst + (int64_t)cb * g.mp + ca) = acc[i][j];
+    }
+}
+
+__global__ void __launch_bounds__(256) ns_join_kernel(NsArgs p, int ver) {
+  __shared__ float tile[64][65];
+  int id = blockIdx.x;
+  const int k = ns_find(p, id, &NsGroup::join);
+  const NsGroup& g = p.g[k];
+  const int nt = g.mp / 64, tri = nt * (nt + 1) / 2, mi = id / tri;
+  int ti, tj;
+  ns_tri(id % tri, nt, ti, tj);
+  const float* src = reinterpret_cast<const float*>(ns_x(p, g, mi, ver ^ 1));
+  uint16_t* dst = ns_sq(p, g, mi, kA);
+  const int lr = threadIdx.x >> 4, lc = (threadIdx.x & 15) * 4, r0 = ti * 64, c0 = tj * 64;
+  const int64_t mm = (int64_t)g.mp * g.mp;
+  nt_f32x4 s[4] = {};
+  for (int sp = 0; sp < g.splits; ++sp)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      s[q] += *reinterpret_cast<const nt_f32x4*>(src + sp * mm + (int64_t)(r0 + lr + 16 * q) * g.mp + c0 + lc);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[lr + 16 * q][lc + e] = s[q][e] * (1.f / kNsX);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int a = lr + 16 * q;
+    float v[4], t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e] = tile[lc + e][a];
+      v[e] = ti == tj && lc + e < a ? t[e] : tile[a][lc + e];  // (a diagonal tile: its upper half both ways)
+    }
+    st4_pair(dst + ns_at(r0 + a, g.mp, c0 + lc), v);
+    if (ti != tj) st4_pair(dst + ns_at(c0 + a, g.mp, r0 + lc), t);
+  }
+}
+
 // The m x m products of a group of steps in one block, for mp <= kNsChain: A (from kA) to P0, or with `two` to Q = P1 P0,
 // in slot kQ.  Two matrices of LDS, in the layout of a K tile of the products above, K tile after K tile: s0 holds A, then
 // T = P0 A, A' = T P0 and P1; s1 holds P0.  A product's 16 x 16 tiles on and above the diagonal are dealt to the 16
@@ -526,6 +591,22 @@ int ns_pick(const NsGroup* g, int ng, NsLaunch what) {
   return best;
 }
 
+// Whether to cut the K of X X^T into runs (64 x 64 tiles), and into how many: as many as fill the chip, of at least 16
+// K tiles each.  The second launch takes about 5 us.
+bool ns_cut(NsGroup* g, int ng) {
+  int blocks = 0;
+  for (int i = 0; i < ng; ++i) blocks += ns_tiles(g[i], 64, kLaunchGram);
+  int whole = 0, longest = 0;
+  for (int i = 0; i < ng; ++i) {
+    const int nk = g[i].np / 32, s = std::max(1, std::min({kNsTiles[0].slots / blocks, g[i].np / g[i].mp, nk / 16}));
+    g[i].run_k = (nk + s - 1) / s;
+    g[i].splits = (nk + g[i].run_k - 1) / g[i].run_k;
+    whole = std::max(whole, nk);
+    longest = std::max(longest, g[i].run_k);
+  }
+  return (whole - longest) * kNsTiles[0].alone > 6.0;
+}
+
 template <class F>
 void ns_with_tile(int t, F f) {
   if (t == 0) f(Tile64());
@@ -577,7 +658,8 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     return a.np != b.np ? a.np > b.np : a.mp > b.mp;
   });
   const int tg = ns_pick(p.g, ng, kLaunchGram), ts = ns_pick(p.g, ng, kLaunchSym), tr = ns_pick(p.g, ng, kLaunchRect);
-  int ew = 0, init = 0, gram = 0, sym = 0, rect = 0, chain = 0;
+  const bool cut = tg == 0 && ns_cut(p.g, ng);
+  int ew = 0, init = 0, gram = 0, sym = 0, rect = 0, chain = 0, join = 0;
   int64_t wat = 0;
   for (int k = 0; k < ng; ++k) {
     NsGroup& g = p.g[k];
@@ -588,11 +670,13 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     g.sym = sym;
     g.rect = rect;
     g.chain = chain;
+    g.join = join;
     chain += g.count;
+    join += ns_tiles(g, 64, kLaunchGram);
     wat += ns_ws_elements(g);
     ew += g.count * g.parts;
     init += g.count * (g.mp / 64) * (g.np / 64);
-    gram += ns_tiles(g, kNsTiles[tg].size, kLaunchGram);
+    gram += ns_tiles(g, kNsTiles[tg].size, kLaunchGram) * (cut ? g.splits : 1);
     sym += ns_tiles(g, kNsTiles[ts].size, kLaunchSym);
     rect += ns_tiles(g, kNsTiles[tr].size, kLaunchRect);
   }
@@ -603,7 +687,12 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
   int ver = 0;
   for (int done = 0; done < steps; ver ^= 1) {
     const bool two = steps - done >= 2;
-    ns_sym<kGram>(p, tg, gram, ver, 0, kA, st);
+    if (cut) {
+      ns_gram_part_kernel<Tile64><<<gram, Tile64::THREADS, 0, st>>>(p, ver);
+      ns_join_kernel<<<join, 256, 0, st>>>(p, ver);
+    } else {
+      ns_sym<kGram>(p, tg, gram, ver, 0, kA, st);
+    }
     if (chained) {
       ns_chain_kernel<<<chain, 1024, 0, st>>>(p, two);
     } else {

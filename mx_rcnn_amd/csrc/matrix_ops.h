@@ -19,7 +19,8 @@ struct NsGroup {
   int64_t run;
   float scale;  // sqrt(max(1, rows / cols)), the update's
   // filled per launch: first matrix, workspace offset (fp16 elements), first work item of each pass
-  int first, ew, init, gram, sym, rect, chain;
+  int first, ew, init, gram, sym, rect, chain, join;
+  int splits, run_k;  // X X^T: runs of K, K tiles of a run
   int64_t ws;
 };
 

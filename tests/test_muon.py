@@ -134,6 +134,21 @@ def test_orthogonalize_strided(dev, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('kind', ['noise', 'power', 'steep'])
+@pytest.mark.parametrize('b,r,c', [(1, 60, 4500), (2, 3001, 70), (1, 129, 2500), (1, 300, 2400), (3, 128, 2050)])
+def test_orthogonalize_long_rows(cuda, kind, b, r, c):
+    """Few matrices with long rows: the sums of X X^T are cut into runs."""
+    g = _matrix(b, r, c, kind, seed=b)
+    _check(ops.orthogonalize(g.to(cuda)), g)
+
+
+@pytest.mark.gpu
+def test_muon_update_long_and_short(cuda):
+    mats = ((0, 64, 3000), (64 * 3000, 30, 20), (64 * 3000 + 600, 2500, 100), (64 * 3000 + 600 + 250000, 64, 64))
+    _check_update(cuda, mats, 64 * 3000 + 600 + 250000 + 4096)
+
+
+@pytest.mark.gpu
 def test_orthogonalize_many_equals_one_by_one(cuda):
     """More matrices than one launch carries, each with the bits that it has alone."""
     g = _matrix(131, 20, 45, 'noise').to(cuda)
