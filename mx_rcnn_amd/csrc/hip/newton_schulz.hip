@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(C::THREADS) ns_gram_part_kernel(NsArgs p, int 
     for (int j = 0; j < C::TB; ++j) {
       if (!C::mine(i, j)) continue;
       const int ca = a0 + (wa * C::TA + i) * 16 + (lane >> 4) * 4, cb = b0 + (wb * C::TB + j) * 16 + (lane & 15);
+      if (ca >= g.mp || cb >= g.mp) continue;
       *reinterpret_cast<nt_f32x4*>(dst + (int64_t)cb * g.mp + ca) = acc[i][j];
     }
 }
@@ -554,57 +555,74 @@ enum NsLaunch { kLaunchGram, kLaunchSym, kLaunchRect };
 
 int ns_tiles(const NsGroup& g, int size, NsLaunch what) {
   const int mt = (g.mp + size - 1) / size, nt = (g.np + size - 1) / size;
-  return g.count * (what == kLaunchRect ? mt * nt : mt * (mt + 1) / 2);
+  return g.count * (what == kLaunchRect ? mt * nt : mt * (mt + 1) / 2 * (what == kLaunchGram ? g.splits : 1));
 }
 
-// The tile for one kind of launch: the groups' tiles dealt out in rounds, longest K first.
-int ns_pick(const NsGroup* g, int ng, NsLaunch what) {
-  int best = 0;
-  double least = 1e30;
-  for (int t = 0; t < 4; ++t) {
-    const NsTile& c = kNsTiles[t];
-    double us = 0;
-    int filled = 0, k_round = 0;
-    for (int i = 0; i < ng; ++i) {
-      const int k = (what == kLaunchGram ? g[i].np : g[i].mp) / 32;
-      for (int n = ns_tiles(g[i], c.size, what); n > 0;) {
-        if (filled == 0) k_round = 0;
-        k_round = std::max(k_round, k);
-        const int take = std::min(n, c.slots - filled);
-        n -= take;
-        filled += take;
-        if (filled == c.slots) {
-          us += k_round * c.full + c.round;
-          filled = 0;
-          // whole rounds of this group alone
-          us += (n / c.slots) * (k * c.full + c.round);
-          n %= c.slots;
-        }
+// Microseconds of one launch: the groups' tiles dealt out in rounds.
+double ns_cost(const NsGroup* g, int ng, const NsTile& c, NsLaunch what) {
+  double us = 0;
+  int filled = 0, k_round = 0;
+  for (int i = 0; i < ng; ++i) {
+    const int k = what == kLaunchGram ? g[i].run_k : g[i].mp / 32;
+    for (int n = ns_tiles(g[i], c.size, what); n > 0;) {
+      if (filled == 0) k_round = 0;
+      k_round = std::max(k_round, k);
+      const int take = std::min(n, c.slots - filled);
+      n -= take;
+      filled += take;
+      if (filled == c.slots) {
+        us += k_round * c.full + c.round;
+        filled = 0;
+        // whole rounds of this group alone
+        us += (n / c.slots) * (k * c.full + c.round);
+        n %= c.slots;
       }
     }
-    if (filled > 0) us += k_round * (c.alone + (c.full - c.alone) * filled / c.slots) + c.round;
-    if (us < least) {
-      least = us;
-      best = t;
-    }
   }
+  if (filled > 0) us += k_round * (c.alone + (c.full - c.alone) * filled / c.slots) + c.round;
+  return us;
+}
+
+int ns_pick(const NsGroup* g, int ng, NsLaunch what) {
+  int best = 0;
+  for (int t = 1; t < 4; ++t)
+    if (ns_cost(g, ng, kNsTiles[t], what) < ns_cost(g, ng, kNsTiles[best], what)) best = t;
   return best;
 }
 
-// Whether to cut the K of X X^T into runs (64 x 64 tiles), and into how many: as many as fill the chip, of at least 16
-// K tiles each.  The second launch takes about 5 us.
-bool ns_cut(NsGroup* g, int ng) {
-  int blocks = 0;
-  for (int i = 0; i < ng; ++i) blocks += ns_tiles(g[i], 64, kLaunchGram);
-  int whole = 0, longest = 0;
+// Cuts X X^T into runs of about `cap` K tiles (as far as the unused version of X holds their sums) -> microseconds
+// of the launch that joins them.
+double ns_cut(NsGroup* g, int ng, int cap) {
+  double bytes = 0;
+  bool any = false;
   for (int i = 0; i < ng; ++i) {
-    const int nk = g[i].np / 32, s = std::max(1, std::min({kNsTiles[0].slots / blocks, g[i].np / g[i].mp, nk / 16}));
+    const int nk = g[i].np / 32, s = std::max(1, std::min(g[i].np / g[i].mp, (nk + cap - 1) / cap));
     g[i].run_k = (nk + s - 1) / s;
     g[i].splits = (nk + g[i].run_k - 1) / g[i].run_k;
-    whole = std::max(whole, nk);
-    longest = std::max(longest, g[i].run_k);
+    any |= g[i].splits > 1;
+    bytes += (double)g[i].count * g[i].mp * g[i].mp * 4 * (g[i].splits + 1);  // (written and read: the upper half)
   }
-  return (whole - longest) * kNsTiles[0].alone > 6.0;
+  return any ? 5 + bytes / 4.5e6 : 0;
+}
+
+// The tile of X X^T and the runs of its K.  (ResNet-101's matrices: 126 us uncut, of which 80 are one 64 x 64 tile of
+// 512 x 9216.)
+int ns_pick_gram(NsGroup* g, int ng, bool& cut) {
+  constexpr int kWhole = 1 << 20;
+  int tile = 0, runs = kWhole;
+  double least = 1e30;
+  for (int cap : {kWhole, 128, 64, 32, 16}) {
+    const double join = ns_cut(g, ng, cap);
+    const int t = ns_pick(g, ng, kLaunchGram);
+    const double us = ns_cost(g, ng, kNsTiles[t], kLaunchGram) + join;
+    if (us < least) {
+      least = us;
+      tile = t;
+      runs = cap;
+    }
+  }
+  cut = ns_cut(g, ng, runs) > 0;
+  return tile;
 }
 
 template <class F>
@@ -657,8 +675,8 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
   std::stable_sort(p.g, p.g + ng, [](const NsGroup& a, const NsGroup& b) {
     return a.np != b.np ? a.np > b.np : a.mp > b.mp;
   });
-  const int tg = ns_pick(p.g, ng, kLaunchGram), ts = ns_pick(p.g, ng, kLaunchSym), tr = ns_pick(p.g, ng, kLaunchRect);
-  const bool cut = tg == 0 && ns_cut(p.g, ng);
+  bool cut;
+  const int tg = ns_pick_gram(p.g, ng, cut), ts = ns_pick(p.g, ng, kLaunchSym), tr = ns_pick(p.g, ng, kLaunchRect);
   int ew = 0, init = 0, gram = 0, sym = 0, rect = 0, chain = 0, join = 0;
   int64_t wat = 0;
   for (int k = 0; k < ng; ++k) {
@@ -672,11 +690,11 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     g.chain = chain;
     g.join = join;
     chain += g.count;
-    join += ns_tiles(g, 64, kLaunchGram);
+    join += ns_tiles(g, 64, kLaunchSym);
     wat += ns_ws_elements(g);
     ew += g.count * g.parts;
     init += g.count * (g.mp / 64) * (g.np / 64);
-    gram += ns_tiles(g, kNsTiles[tg].size, kLaunchGram) * (cut ? g.splits : 1);
+    gram += ns_tiles(g, kNsTiles[tg].size, kLaunchGram);
     sym += ns_tiles(g, kNsTiles[ts].size, kLaunchSym);
     rect += ns_tiles(g, kNsTiles[tr].size, kLaunchRect);
   }
@@ -688,7 +706,10 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
   for (int done = 0; done < steps; ver ^= 1) {
     const bool two = steps - done >= 2;
     if (cut) {
-      ns_gram_part_kernel<Tile64><<<gram, Tile64::THREADS, 0, st>>>(p, ver);
+      ns_with_tile(tg, [&](auto c) {
+        using C = decltype(c);
+        ns_gram_part_kernel<C><<<gram, C::THREADS, 0, st>>>(p, ver);
+      });
       ns_join_kernel<<<join, 256, 0, st>>>(p, ver);
     } else {
       ns_sym<kGram>(p, tg, gram, ver, 0, kA, st);
