@@ -15,6 +15,10 @@
 namespace mxr {
 namespace {
 
+// a launch has fewer than 2^32 threads: blocks of at most 512, and rows of at most 1024 threads each
+constexpr double kInt8Blocks = 1 << 22;
+constexpr int64_t kInt8RowsPerLaunch = 1 << 21;
+
 // ---- rows to 8 bits -----------------------------------------------------------------------------
 // bits of |v|: as integers these order like the values, with infinities and NaN on top
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -171,10 +175,11 @@ __device__ __forceinline__ uint4 load16_tail(const int8_t* row, int k, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows of x (the first `mx` blocks) and of w to 16-byte-aligned copies, `lda` bytes apart, zeros behind K, one behind
-// the other.
-__global__ void __launch_bounds__(256) pack_rows_kernel(Int8Args p, int64_t mx, int8_t* __restrict__ y, int lda) {
-  const int64_t row = blockIdx.x;
+// Rows of x (the first `mx`) and of w to 16-byte-aligned copies, `lda` bytes apart, zeros behind K, one behind the
+// other; from row r0 on, a block each.
+__global__ void __launch_bounds__(256) pack_rows_kernel(Int8Args p, int64_t mx, int64_t r0, int8_t* __restrict__ y,
+                                                        int lda) {
+  const int64_t row = r0 + blockIdx.x;
   const int8_t* src = row < mx ? p.x + row * p.ldx : p.w + (row - mx) * p.ldw;
   for (int k = threadIdx.x * 16; k < lda; k += 4096)
     *reinterpret_cast<uint4*>(y + row * lda + k) = load16_tail(src, k, p.K);
@@ -451,7 +456,7 @@ Int8Plan int8_plan(const Int8Args& a) {
       p.us += pack_us;
       p.pack_bytes = p.bytes = pack_bytes;
     }
-    if (blocks < 2147483647.0 && p.us < best.us) best = p;
+    if (blocks < kInt8Blocks && p.us < best.us) best = p;
   }
   for (int t = 0; t < 3; ++t) {
     const Int8Cand& c = kInt8Tiles[t];
@@ -475,7 +480,7 @@ Int8Plan int8_plan(const Int8Args& a) {
       p.us += pack_us;
       p.pack_bytes = pack_bytes;
       p.bytes = pack_bytes + (splits > 1 ? splits * a.M * a.N * 4 : 0);
-      if (blocks < 2147483647.0 && p.us < best.us) best = p;
+      if (blocks < kInt8Blocks && p.us < best.us) best = p;
     }
   }
   return best;
@@ -490,9 +495,13 @@ void int8_tiles(const Int8Args& a, const Int8Plan& p, int32_t* part, hipStream_t
 
 void quantize_rows(const void* x, int code, int64_t rows, int64_t ld, int K, int8_t* q, int ldq, float* scale,
                    hipStream_t st) {
-  if (code == 0) quantize<0>(x, rows, ld, K, q, ldq, scale, st);
-  else if (code == 1) quantize<1>(x, rows, ld, K, q, ldq, scale, st);
-  else quantize<2>(x, rows, ld, K, q, ldq, scale, st);
+  for (int64_t at = 0; at < rows; at += kInt8RowsPerLaunch) {
+    const int64_t n = std::min(rows - at, kInt8RowsPerLaunch);
+    const char* from = static_cast<const char*>(x) + at * ld * (code == 0 ? 4 : 2);
+    if (code == 0) quantize<0>(from, n, ld, K, q + at * ldq, ldq, scale + at, st);
+    else if (code == 1) quantize<1>(from, n, ld, K, q + at * ldq, ldq, scale + at, st);
+    else quantize<2>(from, n, ld, K, q + at * ldq, ldq, scale + at, st);
+  }
 }
 
 int64_t int8_matmul_ws(const Int8Args& a) { return int8_plan(a).bytes; }
@@ -503,7 +512,8 @@ void int8_matmul(const Int8Args& args, void* ws, hipStream_t st) {
   if (p.pack) {
     int8_t* xb = static_cast<int8_t*>(ws);
     const int64_t mx = int8_x_aligned(a) ? 0 : a.M, nw = int8_w_aligned(a) ? 0 : a.N;
-    pack_rows_kernel<<<(unsigned)(mx + nw), 256, 0, st>>>(a, mx, xb, p.lda);
+    for (int64_t r0 = 0; r0 < mx + nw; r0 += kInt8RowsPerLaunch)
+      pack_rows_kernel<<<(unsigned)std::min(mx + nw - r0, kInt8RowsPerLaunch), 256, 0, st>>>(a, mx, r0, xb, p.lda);
     if (mx > 0) {
       a.x = xb;
       a.ldx = p.lda;

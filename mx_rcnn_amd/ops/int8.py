@@ -77,7 +77,7 @@ def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16)
 
 def int8_linear(x, wq, ws, bias=None, relu=False):
     """A fully connected layer on floating rows ``x`` (M, K) with an 8-bit weight (``quantize_rows`` of the
-    (N, K) weight): the rows quantized, multiplied, scaled back; result in x's type."""
+    (N, K) weight): the rows quantized, multiplied, scaled back; result in x's type.  Not differentiable."""
     if x.is_cuda:  # one call; the rows are quantized into the layout that the product reads
         if x.dim() == 2 and x.shape[1] > MAX_K:
             raise ValueError('int8_linear: K = %d (int32 sums are exact up to %d)' % (x.shape[1], MAX_K))

@@ -170,6 +170,25 @@ def test_int8_matmul_any_address(cuda, M, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('K', [5, 9, 100])
+def test_more_rows_than_one_launch_takes(cuda, K):
+    """Rows past 2^21 (quantized, copied) and 2^22 blocks: the last ones are as if they were alone."""
+    M = (1 << 22) + 77
+    gen = torch.Generator(device='cuda').manual_seed(K)
+    x = torch.randn(M, K, generator=gen, device=cuda, dtype=torch.bfloat16)
+    q, s = ops.quantize_rows(x)
+    wq, ws = ops.quantize_rows(torch.randn(40, K, generator=gen, device=cuda))
+    y = ops.int8_matmul(q, s, wq, ws)
+    y2 = ops.int8_linear(x, wq, ws)
+    for at in (0, (1 << 21) - 3, (1 << 22) - 3, M - 30):
+        part = slice(at, at + 30)
+        q1, s1 = ops.quantize_rows(x[part])
+        assert torch.equal(q[part], q1) and torch.equal(s[part], s1), at
+        want = ops.int8_matmul(q1, s1, wq, ws)
+        assert torch.equal(y[part], want) and torch.equal(y2[part], want), at
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
 def test_int8_linear_is_its_two_parts(cuda, dtype):
     gen = torch.Generator().manual_seed(4)
