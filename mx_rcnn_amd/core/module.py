@@ -26,6 +26,7 @@ from ..parallel import dist as pdist
 from ..parallel import watchdog
 from .callback import BatchEndParam
 from .lr_scheduler import FactorScheduler
+from .params import is_muon_matrix
 from .trainer import GraphedStep, Trainer
 from ..utils import profiler as prof
 
@@ -331,6 +332,8 @@ class MutableModule(object):
         """Momentum + update count (MXNet ``Module.save_optimizer_states``), MXNet .params codec."""
         from ..utils import ndarray_io
         st = {'mom:' + k: v.detach().cpu().numpy() for k, v in self.trainer.store.optimizer_state().items()}
+        if self.trainer.optimizer == 'muon':
+            st['muon'] = np.ones(1, np.float32)
         st['num_update'] = np.array([self.trainer.num_update], np.float32)
         st['rng_step'] = self.trainer.rng_step.detach().cpu().numpy().astype(np.float64)  # dropout counter
         st['rng_cpu'] = torch.get_rng_state().numpy()
@@ -342,6 +345,9 @@ class MutableModule(object):
         from ..utils import ndarray_io
         st = ndarray_io.load(fname)
         moms = {k[4:]: v for k, v in st.items() if k.startswith('mom:')}
+        if ('muon' in st) != (self.trainer.optimizer == 'muon'):
+            # sgd's momentum holds steps (- lr * gradient), muon's gradients: its matrices start from zero
+            moms = {k: v for k, v in moms.items() if not is_muon_matrix(k, v.shape)}
         missing = self.trainer.store.load_optimizer_state(moms)
         if 'num_update' in st:
             self.trainer.num_update = int(np.asarray(st['num_update']).reshape(-1)[0])

@@ -33,6 +33,11 @@ from ..ops import precision
 MUON_EXCLUDE = ('rpn_cls_score', 'rpn_bbox_pred', 'cls_score', 'bbox_pred')
 
 
+def is_muon_matrix(name, shape):
+    """Whether the Muon optimizer updates this parameter: a conv / FC weight that is no predictor's."""
+    return name.endswith('_weight') and len(shape) >= 2 and name[:-len('_weight')] not in MUON_EXCLUDE
+
+
 def _is_bn_param(name):
     return name.endswith('_gamma') or name.endswith('_beta')
 
@@ -464,7 +469,7 @@ class FlatParamStore:
         for gi, g in enumerate(self.groups):
             mats = []
             for (n, _, _, numel, shape, cl), off in zip(g.entries, g.offsets):
-                if n.endswith('_weight') and len(shape) >= 2 and n[:-len('_weight')] not in MUON_EXCLUDE:
+                if is_muon_matrix(n, shape):
                     mats.append((off, shape[0], numel // shape[0]))
                     names.append(n)
             if mats:

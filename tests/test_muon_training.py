@@ -112,6 +112,35 @@ def test_step_cpu():
     assert torch.equal(after['stage1_unit1_conv1_weight'], before['stage1_unit1_conv1_weight'])
 
 
+def test_states_of_the_other_optimizer(tmp_path):
+    """A states file restores the momentum of its own optimizer; of the other one's, all but the matrices'."""
+    from tests.test_observability import _tiny_module
+    opt = {'learning_rate': 1e-3, 'momentum': 0.9, 'wd': 5e-4}
+    files = {}
+    for name in ('sgd', 'muon'):
+        torch.manual_seed(3)
+        mod, data = _tiny_module()
+        files[name] = str(tmp_path / name) + '-0001.states'
+        mod.fit(data, num_epoch=1, states_prefix=str(tmp_path / name), optimizer=name, optimizer_params=opt)
+        if name == 'muon':
+            names = mod.trainer.muon_names
+            assert names
+        kept = {k: v.clone() for k, v in mod.trainer.store.optimizer_state().items()}
+        for other in ('sgd', 'muon'):
+            mod2, _ = _tiny_module()
+            mod2.init_optimizer(optimizer=other, optimizer_params=opt)
+            if other == name:
+                mod2.load_optimizer_states(files[name])
+                for k, v in mod2.trainer.store.optimizer_state().items():
+                    assert torch.equal(v, kept[k]), k
+    for name, other in (('sgd', 'muon'), ('muon', 'sgd')):
+        mod2, _ = _tiny_module()
+        mod2.init_optimizer(optimizer=other, optimizer_params=opt)
+        mod2.load_optimizer_states(files[name])
+        for k, v in mod2.trainer.store.optimizer_state().items():
+            assert bool(v.any()) != (k in names), (name, k)
+
+
 def _worker(rank, world, port, out_dir):
     os.environ.update({'MASTER_ADDR': '127.0.0.1', 'MASTER_PORT': str(port), 'RANK': str(rank),
                        'WORLD_SIZE': str(world), 'LOCAL_RANK': str(rank)})
