@@ -53,6 +53,9 @@ def parse_args(argv=None):
     ap.add_argument('--train-mode', default='e2e', choices=['e2e', 'rpn', 'rcnn'],
                     help='e2e (headline) or one stage of 4-step alternate training (BASELINE config 4): '
                          'rpn = RPN-only step, rcnn = Fast R-CNN step on 128 given RoIs per image')
+    ap.add_argument('--optimizer', default='sgd', choices=['sgd', 'muon'],
+                    help='sgd (headline), or muon: conv / FC weights but the predictors step along their '
+                         'orthogonalised momentum (ops/muon.py)')
     return ap.parse_args(argv)
 
 
@@ -196,7 +199,8 @@ def run(args, precision, rank, world, device):
     fixed = ['conv0', 'stage1', 'stage2', 'bn_data', 'bn0'] if args.network.startswith('resnet') else ['conv1', 'conv2']
     trainer = Trainer(model, args.train_mode, fixed_param_prefix=fixed, lr=0.001, momentum=0.9, wd=0.0005, clip_gradient=1.0,
                       rescale_grad=1.0, device=device, bucket_mb=args.bucket_mb, precision=precision,
-                      grad_comm_dtype=torch.float32 if args.grad_comm == 'fp32' else torch.bfloat16)
+                      grad_comm_dtype=torch.float32 if args.grad_comm == 'fp32' else torch.bfloat16,
+                      optimizer=args.optimizer)
 
     mode = args.mode if device.type == 'cuda' else 'eager'
     step_fn = None
@@ -264,7 +268,7 @@ def run(args, precision, rank, world, device):
                h, w, 'float' if args.host_float_data else 'uint8 BGR (raw-loader form, converted in the step)'),
            'config': {'model': '%s-faster-rcnn%s' % (args.network, '-c4' if args.network.startswith('resnet') else ''), 'global_batch': args.ims_per_gpu * world,
                       'seq_len': None, 'image_hw': [h, w], 'num_classes': args.num_classes,
-                      'ims_per_gpu': args.ims_per_gpu, 'train_mode': args.train_mode, 'parallelism': 'dp%d' % world,
+                      'ims_per_gpu': args.ims_per_gpu, 'train_mode': args.train_mode, 'optimizer': args.optimizer, 'parallelism': 'dp%d' % world,
                       'precision': PRECISION_NOTE.get(trainer.precision, trainer.precision),
                       'rpn_pre_post_nms': [cfg.TRAIN.RPN_PRE_NMS_TOP_N, cfg.TRAIN.RPN_POST_NMS_TOP_N],
                       'rois_per_image': cfg.TRAIN.BATCH_SIZE, 'exec': mode,
