@@ -695,10 +695,14 @@ static void ns_dispatch(const std::vector<std::array<int64_t, 3>>& mats, const m
       ws += mxr::ns_ws_elements(g);
       groups.push_back(g);
     }
-    Tensor buf = at::empty({ws}, o.dtype(at::kHalf));
-    Tensor part = at::empty({(int64_t)off.size() * mxr::kNsParts}, o.dtype(at::kDouble));
+    Tensor buf, part;
+    if (!mxr::ns_in_blocks(groups.data(), (int)groups.size())) {
+      buf = at::empty({ws}, o.dtype(at::kHalf));
+      part = at::empty({(int64_t)off.size() * mxr::kNsParts}, o.dtype(at::kDouble));
+    }
     mxr::ns_run(groups.data(), (int)groups.size(), off.data(), (int)off.size(), u, (int)steps,
-                reinterpret_cast<uint16_t*>(buf.data_ptr()), part.data_ptr<double>(), cur_stream());
+                buf.defined() ? reinterpret_cast<uint16_t*>(buf.data_ptr()) : nullptr,
+                part.defined() ? part.data_ptr<double>() : nullptr, cur_stream());
     LAUNCH_CHECK("newton_schulz");
     at = end;
   }

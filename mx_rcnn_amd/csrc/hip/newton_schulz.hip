@@ -474,6 +474,147 @@ __global__ void __launch_bounds__(1024) ns_chain_kernel(NsArgs p, int two) {
   product(s0, s1, nullptr, false);
 }
 
+// ---- a matrix in one block -----------------------------------------------------------------------
+// Matrices of at most 64 in the small dimension and kNsBlockX elements go through all steps in one block's LDS, in one
+// launch, in fp32 on the fp32 matrix instructions: X (pm x pn, both padded to 16), A and P.  Launches and their latency, not
+// products, are what such matrices cost otherwise; and the steps run one by one, since few and short sums leave the plain
+// recurrence in fp32 so exact that gathering them was up to 2.2 times further off (8 x 8, 64 x 12).
+// In a block / by launches, us: 8 x 8 10 / 60, 64 x 64 27 / 62, 64 x 256 57 / 68, 64 x 320 68 / 69, 64 x 400 85 / 71, 48 x 400
+// 58 / 71, 30 x 600 49 / 74, 16 x 1200 60 / 81, 100 of 64 x 64 27 / 70.
+constexpr int kNsBlockX = 20992;
+constexpr int kNsBlockFloats = kNsBlockX + 64 * 4 + 2 * 64 * 68;
+__host__ __device__ __forceinline__ int ns_pad16(int n) { return (n + 15) / 16 * 16; }
+
+__global__ void __launch_bounds__(1024) ns_block_kernel(NsArgs p, NsUpdate u, int steps) {
+  __shared__ __attribute__((aligned(16))) float pool[kNsBlockFloats];
+  __shared__ double red[16];
+  int mi = blockIdx.x;
+  const int k = ns_find(p, mi, &NsGroup::chain);
+  const NsGroup& g = p.g[k];
+  const int pm = ns_pad16(g.m), pn = ns_pad16(g.n), lx = pn + 4, la = pm + 4;  // (16 rows: 16 different banks)
+  float *X = pool, *A = X + pm * lx, *P = A + pm * la;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4 << 2;
+  const int64_t off = p.off[g.first + mi];
+  const int total = g.rows * g.cols;
+  for (int i = tid; i < pm * lx; i += 1024) X[i] = 0.f;
+  __syncthreads();
+  const auto place = [&](int i) {  // of element i of the matrix in memory
+    const int r = i / g.cols, c = i - r * g.cols;
+    return g.tall ? c * lx + r : r * lx + c;
+  };
+  double s = 0.0;
+  for (int i = tid; i < total; i += 1024) {
+    float v = ns_grad(u, off + i);
+    if (u.mom != nullptr) {
+      const float m = u.mu * u.mom[off + i] + v;
+      u.mom[off + i] = m;
+      v = u.nesterov ? v + u.mu * m : m;
+    }
+    if (u.zero != nullptr) st(u.zero, off + i, 0.f, u.zero_code);
+    X[place(i)] = v;
+    s += (double)v * (double)v;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += red[w];
+  const double f = 1.0 / (sqrt(s) + u.eps);
+  for (int i = tid; i < pm * lx; i += 1024) X[i] = (float)((double)X[i] * f);
+  __syncthreads();
+
+  // Of 16 consecutive k a lane holds the four of its group for its row of either operand: four matrix instructions, each
+  // over one k of every group.
+  const auto mma4 = [](const float4& a, const float4& b, nt_f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
+  };
+  // dst (pm x pm) = L L^T over nk columns, or a I + b L + c L L^T: at most 10 tiles on and above the diagonal, a wave
+  // each, every value written to both of its places.  Sums in runs of 64 k.
+  const int nt = pm / 16;
+  const auto product = [&](const float* L, int ld, int nk, float* dst, bool poly) {
+    int ti = 0, tj = 0;
+    const bool mine = wave < nt * (nt + 1) / 2;
+    nt_f32x4 sum = {0, 0, 0, 0};
+    if (mine) {
+      ns_tri(wave, nt, ti, tj);
+      const float *a = L + (tj * 16 + r16) * ld + g4, *b = L + (ti * 16 + r16) * ld + g4;
+      int k0 = 0;
+      for (; k0 + 64 <= nk; k0 += 64) {
+        nt_f32x4 acc = {0, 0, 0, 0};
+        float4 x[4], y[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          x[q] = *reinterpret_cast<const float4*>(a + k0 + 16 * q);
+          y[q] = *reinterpret_cast<const float4*>(b + k0 + 16 * q);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc = mma4(x[q], y[q], acc);
+        sum += acc;
+      }
+      nt_f32x4 acc = {0, 0, 0, 0};
+      for (; k0 < nk; k0 += 16)
+        acc = mma4(*reinterpret_cast<const float4*>(a + k0), *reinterpret_cast<const float4*>(b + k0), acc);
+      sum += acc;
+    }
+    __syncthreads();
+    if (mine) {
+      const int row = ti * 16 + r16, col = tj * 16 + g4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (col + e < row) continue;
+        const float v = poly ? (col + e == row ? kNsA : 0.f) + kNsB * L[row * la + col + e] + kNsC * sum[e] : sum[e];
+        dst[row * la + col + e] = v;
+        dst[(col + e) * la + row] = v;
+      }
+    }
+    __syncthreads();
+  };
+  for (int step = 0; step < steps; ++step) {
+    product(X, lx, pn, A, false);
+    product(A, la, pm, P, true);
+    // X = P X in place: a wave reads and writes whole columns, 16 at a time
+    for (int c0 = wave * 16; c0 < pn; c0 += 256) {
+      nt_f32x4 acc[4] = {};
+      float4 b[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < nt) {
+          const float* x = X + (q * 16 + g4) * lx + c0 + r16;
+          b[q] = make_float4(x[0], x[lx], x[2 * lx], x[3 * lx]);
+        }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (q < nt && i < nt)
+            acc[i] = mma4(*reinterpret_cast<const float4*>(P + (i * 16 + r16) * la + q * 16 + g4), b[q], acc[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) X[(i * 16 + g4 + e) * lx + c0 + r16] = acc[i][e];
+        }
+    }
+    __syncthreads();
+  }
+  const float lr = u.lr != nullptr ? *u.lr : 0.f;
+  for (int i = tid; i < total; i += 1024) {
+    float v = X[place(i)];
+    if (u.w != nullptr) {
+      const float w = u.w[off + i];
+      v = w - lr * (g.scale * v + u.wd * w);
+    }
+    st(u.out, off + i, v, u.out_code);
+    if (u.shadow != nullptr) stc(u.shadow, off + i, v, u.shadow_code, u.shadow_plane);
+  }
+}
+
 // X' = Q X, X read across its lines (TURN), so that it need not be kept both ways: writing X^T beside X took 36 of 52 us
 // at 23 x 256 x 2304.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X' is the
 // other version of X for the next group of steps.
@@ -658,6 +799,13 @@ void ns_shape(NsGroup& g) {
 
 int64_t ns_ws_elements(const NsGroup& g) { return g.count * ns_stride(g); }
 
+bool ns_in_blocks(const NsGroup* g, int ng) {
+  return std::all_of(g, g + ng, [](const NsGroup& g) {
+    const int pm = ns_pad16(g.m), pn = ns_pad16(g.n);
+    return g.m <= 64 && (int64_t)pm * pn <= kNsBlockX;
+  });
+}
+
 void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const NsUpdate& u, int steps, uint16_t* ws,
             double* part, hipStream_t st) {
   NsArgs p = {};
@@ -670,6 +818,15 @@ void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const 
     p.g[k] = groups[k];
     p.g[k].first = at;
     at += groups[k].count;
+  }
+  if (ns_in_blocks(p.g, ng)) {
+    int blocks = 0;
+    for (int k = 0; k < ng; ++k) {
+      p.g[k].chain = blocks;
+      blocks += p.g[k].count;
+    }
+    ns_block_kernel<<<blocks, 1024, 0, st>>>(p, u, steps);
+    return;
   }
   // long products first
   std::stable_sort(p.g, p.g + ng, [](const NsGroup& a, const NsGroup& b) {

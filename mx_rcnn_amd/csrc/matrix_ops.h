@@ -46,6 +46,7 @@ struct NsUpdate {
 
 void ns_shape(NsGroup& g);                     // from count / rows / cols
 int64_t ns_ws_elements(const NsGroup& g);      // fp16 elements of workspace
+bool ns_in_blocks(const NsGroup* g, int ng);   // all of them fit a block each: no workspace
 void ns_run(const NsGroup* groups, int ng, const int64_t* off, int nmats, const NsUpdate& u, int steps, uint16_t* ws,
             double* part, hipStream_t st);
 
