@@ -439,7 +439,8 @@ Int8Plan int8_plan(const Int8Args& a) {
   const int64_t packed = (ax ? 0 : a.M) + (aw ? 0 : a.N);  // rows to copy
   const double pack_us = packed ? 3 + 2 * packed * k / 5e6 : 0;
   const int64_t pack_bytes = (packed * lda + 255) / 256 * 256;
-  for (int s = 0; s < 4; ++s) {  // 16 or 32 rows of x; unaligned rows as they are, or copied first
+  // 16 or 32 rows of x; unaligned rows as they are, or copied first (16 x 4096 x 4099: 8.5 / 20 us, 40 x 64 x 20001: 28 / 16)
+  for (int s = 0; s < 4; ++s) {
     if (s >= 2 && aligned) break;
     if (s < 2 && (a.ldw >= kInt8Ld || a.ldx >= kInt8Ld)) continue;
     Int8Plan p = {};

@@ -22,7 +22,12 @@
 // times larger in the result (2 x 3 matrices, 1e-4).
 //
 // One launch runs a product of every matrix of the call: a block finds its matrix among the groups of
-// equal shape that the launch carries by value (no tables in memory, so a call can be captured).
+// equal shape that the launch carries by value (no tables in memory, so a call can be captured).  Small matrices, bound
+// by launches, take other ways: ns_chain_kernel, and ns_block_kernel for whole matrices.
+//
+// Times on this card (5 steps): 64 x 576 74 us, 23 of 256 x 2304 300 us, 4096 x 4096 3.7 ms; the update of ResNet-101's
+// filters 1.36 ms, of VGG16's 17.0 ms.  4096 x 4096 and VGG16 run at 89 and 85 % of
+// the rate of a large fp16 product.
 #include "tile_nt.h"
 
 #include <algorithm>
@@ -373,10 +378,12 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs p, int ver) {
   }
 }
 
-// The m x m products of a group of steps in one block, for mp <= kNsChain: A (from kA) to P0, or with `two` to Q = P1 P0,
-// in slot kQ.  Two matrices of LDS, in the layout of a K tile of the products above, K tile after K tile: s0 holds A, then
-// T = P0 A, A' = T P0 and P1; s1 holds P0.  A product's 16 x 16 tiles on and above the diagonal are dealt to the 16
-// waves, held in registers until every wave has read its operands, and written with their mirror images.
+// The m x m products of a group of steps in one block, for mp <= kNsChain: A (from kA) to P0, or with `two` to Q = P1
+// P0, in slot kQ.  Two matrices of LDS, in the layout of a K tile of the products above, K tile after K tile: s0
+// holds A, then T = P0 A, A' = T P0 and P1; s1 holds P0.  A product's 16 x 16 tiles on and above the diagonal are
+// dealt to the 16 waves, held in registers until every wave has read its operands, and written with their mirror
+// images.  Five launches of 5 us or more become one of 8 (64 x 576: 116 -> 74 us in all).  Here the lo lo products
+// are taken too: their cost does not show, and small matrices come out 10 to 15 % nearer.
 constexpr int kNsChain = 128;
 
 __device__ __forceinline__ int ns_lds_at(int row, int rows, int col) {  // byte of the hi value; the lo value's is ^ 64
@@ -418,6 +425,7 @@ __global__ void __launch_bounds__(1024) ns_chain_kernel(NsArgs p, int two) {
           x[h] = nt_frag(L + kt * mp * 128, tj[t] * 16 + (lane & 15), h, lane);
           y[h] = nt_frag(R + kt * mp * 128, ti[t] * 16 + (lane & 15), h, lane);
         }
+        acc[t] = nt_mma(x[1], y[1], acc[t]);
         acc[t] = nt_mma(x[0], y[1], acc[t]);
         acc[t] = nt_mma(x[1], y[0], acc[t]);
         acc[t] = nt_mma(x[0], y[0], acc[t]);
@@ -445,7 +453,8 @@ __global__ void __launch_bounds__(1024) ns_chain_kernel(NsArgs p, int two) {
       for (int e = 0; e < 4; ++e) v[e] = acc[t][e] * (poly ? 1.f / (kNsX * kNsX) : 1.f / kNsP);
       if (poly) {
         const int at = ns_lds_at(row, mp, col);
-        const ushort4 h = *reinterpret_cast<const ushort4*>(L + at), l = *reinterpret_cast<const ushort4*>(L + (at ^ 64));
+        const ushort4 h = *reinterpret_cast<const ushort4*>(L + at);
+        const ushort4 l = *reinterpret_cast<const ushort4*>(L + (at ^ 64));
         const float av[4] = {f16_to_f32(h.x) + f16_to_f32(l.x), f16_to_f32(h.y) + f16_to_f32(l.y),
                              f16_to_f32(h.z) + f16_to_f32(l.z), f16_to_f32(h.w) + f16_to_f32(l.w)};
 #pragma unroll
@@ -475,14 +484,15 @@ __global__ void __launch_bounds__(1024) ns_chain_kernel(NsArgs p, int two) {
 }
 
 // ---- a matrix in one block -----------------------------------------------------------------------
-// Matrices of at most 64 in the small dimension and kNsBlockX elements go through all steps in one block's LDS, in one
-// launch, in fp32 on the fp32 matrix instructions: X (pm x pn, both padded to 16), A and P.  Launches and their latency, not
-// products, are what such matrices cost otherwise; and the steps run one by one, since few and short sums leave the plain
-// recurrence in fp32 so exact that gathering them was up to 2.2 times further off (8 x 8, 64 x 12).
-// In a block / by launches, us: 8 x 8 10 / 60, 64 x 64 27 / 62, 64 x 256 57 / 68, 64 x 320 68 / 69, 64 x 400 85 / 71, 48 x 400
-// 58 / 71, 30 x 600 49 / 74, 16 x 1200 60 / 81, 100 of 64 x 64 27 / 70.
-constexpr int kNsBlockX = 20992;
-constexpr int kNsBlockFloats = kNsBlockX + 64 * 4 + 2 * 64 * 68;
+// Matrices of at most 64 in the small dimension and ns_block_x elements go through all steps in one block's LDS, in
+// one launch, in fp32 on the fp32 matrix instructions: X (pm x pn, both padded to 16), A and P.  Launches and their
+// latency, not products, are what such matrices cost otherwise; and the steps run one by one, since few and short
+// sums leave the plain recurrence in fp32 so exact that gathering them was up to 2.2 times further off (8 x 8, 64 x
+// 12). In a block / by launches, us: 8 x 8 10 / 60, 64 x 64 27 / 62, 64 x 256 57 / 68, 64 x 320 68 / 69, 64 x 400 85
+// / 71, 48 x 400 58 / 71, 30 x 600 49 / 74, 30 x 1000 74 / 81, 16 x 1200 60 / 81, 100 of 64 x 64 27 / 70.
+__host__ __device__ constexpr int ns_block_x(int pm) { return pm > 32 ? 20992 : 28800; }
+constexpr int kNsBlockFloats =
+    std::max(ns_block_x(64) + 64 * 4 + 2 * 64 * 68, ns_block_x(32) + 32 * 4 + 2 * 32 * 36);
 __host__ __device__ __forceinline__ int ns_pad16(int n) { return (n + 15) / 16 * 16; }
 
 __global__ void __launch_bounds__(1024) ns_block_kernel(NsArgs p, NsUpdate u, int steps) {
@@ -615,9 +625,9 @@ __global__ void __launch_bounds__(1024) ns_block_kernel(NsArgs p, NsUpdate u, in
   }
 }
 
-// X' = Q X, X read across its lines (TURN), so that it need not be kept both ways: writing X^T beside X took 36 of 52 us
-// at 23 x 256 x 2304.  FINAL: the result leaves as the matrix itself (out) or as the weight update; otherwise X' is the
-// other version of X for the next group of steps.
+// X' = Q X, X read across its lines (TURN), so that it need not be kept both ways: with X^T written beside X, 52 us
+// instead of 41 at 23 x 256 x 2304 (and 24 instead of 17 in pass 2).  FINAL: the result leaves as the matrix itself
+// (out) or as the weight update; otherwise X' is the other version of X for the next group of steps.
 template <class C, bool FINAL>
 __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate u, int ver) {
   __shared__ __attribute__((aligned(1024))) char ring[C::LDS];
@@ -676,10 +686,12 @@ __global__ void __launch_bounds__(C::THREADS) ns_apply_kernel(NsArgs p, NsUpdate
 }
 
 // Tiles and their measured cost: microseconds per K tile with one block per CU alone and with every slot taken, slots
-// (blocks resident on the chip), and microseconds of start and epilogue per round.  Larger tiles read fewer bytes
-// per product, smaller ones fill the chip: 4096 x 4096 (us for a symmetric product / for P X) 64: 330 / 640, 128:
-// 262 / 380, 192: 222 / 410 (253 tiles, one round), 256: 265 (136 tiles on 256 CUs) / 313; ResNet-101's 84
-// matrices 64: 40 / 316, 128: 42 / 211, 192: 65 / 254, 256: 91 / 202.
+// (blocks resident on the chip), and microseconds of start and epilogue per round.  Larger tiles read fewer bytes per
+// product, smaller ones fill the chip.  Whole runs with one kind of product at 64 / 128 / 192 / 256, us: symmetric m
+// x m products of 4096 x 4096 5580 / 4410 / 3930 / -, of ResNet-101's 84 matrices 1500 / 1390 / - / -, of 23 x 256 x
+// 2304 300 / 392 / - / -; P X of 4096 x 4096 - / 4060 / 4210 / 3920, of ResNet-101 - / 1390 / 1575 / 1383; X X^T of
+// 23 x 256 x 2304 294 / 388 / 514 / 654.  The ring of the 64 x 64 tile holds 4 stages: 2 took 27 instead of 24 us for
+// the last.
 using Tile64 = NtCfg<true, 64, 64, 2, 2, 2, 4, 4, true>;  // two K groups: short products are bound by latency
 using Tile128 = NtCfg<true, 128, 128, 1, 2, 4, 2, 8>;
 using Tile192 = NtCfg<true, 192, 192, 1, 2, 4, 3, 8>;
@@ -802,7 +814,7 @@ int64_t ns_ws_elements(const NsGroup& g) { return g.count * ns_stride(g); }
 bool ns_in_blocks(const NsGroup* g, int ng) {
   return std::all_of(g, g + ng, [](const NsGroup& g) {
     const int pm = ns_pad16(g.m), pn = ns_pad16(g.n);
-    return g.m <= 64 && (int64_t)pm * pn <= kNsBlockX;
+    return g.m <= 64 && (int64_t)pm * pn <= ns_block_x(pm);
   });
 }
 
