@@ -150,8 +150,10 @@ void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, int ldq
     const int per = t < 256 ? 256 / t : 1;
     kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, ldq, scale);
   };
+  // bf16 rows, us, one way and the next: 2048 x 512 2.7 / 2.9 (a wave, 8 values a lane / 32), 2048 x 1024 3.5 / 4.2 but 64 x
+  // 1024 3.1 / 2.7 (a wave / 256 threads), 2048 x 4096 7.3 / 8.1 (256 / 512), 2048 x 8192 11 / 15.5 (16 values / 64),
+  // 2048 x 32768 39 / 50 (held / read twice); 2400 x 25088 with 256 / 512 / 1024 threads per row 36 / 33 / 41 (5.5 TB/s)
   if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, ldq, scale);
-  // 2400 x 25088 bf16 with 256 / 512 / 1024 threads per row: 36 / 33 / 41 us (512: 5.5 TB/s)
   else if (K <= 512) go(quantize_kernel<CODE, 64, 1, true>, 64);
   else if (K <= 2048 && rows >= 2048) go(quantize_kernel<CODE, 64, 4, true>, 64);
   else if (K <= 4096) go(quantize_kernel<CODE, 256, 2, true>, 256);
