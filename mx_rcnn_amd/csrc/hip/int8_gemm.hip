@@ -150,8 +150,8 @@ void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, int ldq
     const int per = t < 256 ? 256 / t : 1;
     kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, ldq, scale);
   };
-  // bf16 rows, us, one way and the next: 2048 x 512 2.7 / 2.9 (a wave, 8 values a lane / 32), 2048 x 1024 3.5 / 4.2 but 64 x
-  // 1024 3.1 / 2.7 (a wave / 256 threads), 2048 x 4096 7.3 / 8.1 (256 / 512), 2048 x 8192 11 / 15.5 (16 values / 64),
+  // bf16 rows, us, one way and the next: 2048 x 512 2.7 / 2.9 (a wave, 8 values a lane / 32), 2048 x 1024 3.5 / 4.2
+  // but 64 x 1024 3.1 / 2.7 (a wave / 256 threads), 2048 x 4096 7.3 / 8.1 (256 / 512), 2048 x 8192 11 / 15.5 (16 values / 64),
   // 2048 x 32768 39 / 50 (held / read twice); 2400 x 25088 with 256 / 512 / 1024 threads per row 36 / 33 / 41 (5.5 TB/s)
   if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, ldq, scale);
   else if (K <= 512) go(quantize_kernel<CODE, 64, 1, true>, 64);
@@ -220,7 +220,7 @@ __device__ __forceinline__ void int8_store(const Int8Args& p, int32_t* part, int
 
 // Few rows of x, or little of everything: each of KG waves reads both operands' fragments of every KG-th K tile
 // straight into registers, two K tiles ahead, with no barrier until the sums of the waves are added up in LDS.  A
-// block has 16 rows of w and 16 TB rows of x.  One row against 4096 x 25088: 19.5 us, 5.3 TB/s.
+// block has 16 rows of w, 16 TB rows of x and one run of K.  One row against 4096 x 25088: 19.5 us, 5.3 TB/s.
 //
 // Rows at any address (ALIGNED = false) need no copy: the 4 or 5 dwords that hold a lane's 16 bytes are loaded and moved
 // down when they are used.  (As one unaligned load they take 5 times as long as an aligned one.)  Behind K the bytes of x
@@ -236,13 +236,14 @@ struct Int8Stream {
   uint32_t ow, ox[TB];  // of this lane's first byte; unaligned: of its dword
   int sw, sx[TB];       // unaligned: the byte within the dword
 
-  __device__ __forceinline__ Int8Stream(const Int8Args& a, int n, int64_t m, int k)
+  // K columns from k_lo on, a multiple of STEP
+  __device__ __forceinline__ Int8Stream(const Int8Args& a, int n, int64_t m, int k_lo, int k)
       : p(a), n0(n), k_hi(k), r(threadIdx.x & 15), ch((threadIdx.x & 63) >> 4 << 4),
         kg(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m) {
     const int wr = min(p.N - n0, 16), xr = (int)min(p.M - m0, (int64_t)16 * TB);
     const int ldw = (int)p.ldw, ldx = (int)p.ldx;  // (below 2^22)
-    const char* w = reinterpret_cast<const char*>(p.w) + n0 * p.ldw;
-    const char* x = reinterpret_cast<const char*>(p.x) + m0 * p.ldx;
+    const char* w = reinterpret_cast<const char*>(p.w) + n0 * p.ldw + k_lo;
+    const char* x = reinterpret_cast<const char*>(p.x) + m0 * p.ldx + k_lo;
     const int w0 = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(w) & 3);
     const int x0 = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(x) & 3);
     rw = nt_rsrc(w - w0, (w0 + (wr - 1) * ldw + k_hi + 3) & ~3);
@@ -319,17 +320,19 @@ struct Int8Stream {
 };
 
 template <int TB, bool ALIGNED>
-__global__ void __launch_bounds__(512) int8_stream_kernel(Int8Args p, int nt, int mt) {
+__global__ void __launch_bounds__(512) int8_stream_kernel(Int8Args p, int nt, int mt, int splits, int run,
+                                                         int32_t* __restrict__ part) {
   using S = Int8Stream<TB, ALIGNED>;
   __shared__ nt_i32x4 sums[S::KG][TB][64];
-  const int id = nt_xcd_item(blockIdx.x, nt * mt), lane = threadIdx.x & 63;
-  const S s(p, id / mt * 16, (int64_t)(id % mt) * 16 * TB, p.K);
+  const int id = nt_xcd_item(blockIdx.x, nt * mt * splits), lane = threadIdx.x & 63;
+  const int sp = id / (nt * mt), t = id % (nt * mt), K = min(run, p.K - sp * run);
+  const S s(p, t / mt * 16, (int64_t)(t % mt) * 16 * TB, sp * run, K);
   constexpr int STEP = S::STEP;
   nt_i32x4 acc[TB];
 #pragma unroll
   for (int j = 0; j < TB; ++j) acc[j] = nt_i32x4{0, 0, 0, 0};
   // whole steps (aligned: all; what is past the end is zeros), and an unaligned rest
-  const int end = ALIGNED ? p.K : p.K / STEP * STEP;
+  const int end = ALIGNED ? K : K / STEP * STEP;
   typename S::Frags f[2], rest;
   if constexpr (!ALIGNED) s.template load<true>(rest, end);
   s.template load<false>(f[0], 0, ALIGNED || 0 < end);
@@ -344,10 +347,10 @@ __global__ void __launch_bounds__(512) int8_stream_kernel(Int8Args p, int nt, in
   for (int j = 0; j < TB; ++j) sums[s.kg][j][lane] = acc[j];
   __syncthreads();
   if (s.kg >= TB) return;
-  nt_i32x4 t = sums[0][s.kg][lane];
+  nt_i32x4 v = sums[0][s.kg][lane];
 #pragma unroll
-  for (int g = 1; g < S::KG; ++g) t += sums[g][s.kg][lane];
-  int8_store(p, nullptr, 1, 0, s.m0 + s.kg * 16 + s.r, s.n0 + s.ch / 4, t);
+  for (int g = 1; g < S::KG; ++g) v += sums[g][s.kg][lane];
+  int8_store(p, part, splits, sp, s.m0 + s.kg * 16 + s.r, s.n0 + s.ch / 4, v);
 }
 
 // One BA (of N) x BB (of M) tile and one run of K per block: the result itself, or with several runs the
@@ -424,6 +427,7 @@ struct Int8Plan {
   double us;
 };
 
+constexpr int kStreamTiles = Int8Stream<1, true>::STEP / 128;
 constexpr int64_t kInt8Ld = 1 << 22;  // rows closer than that: 32-bit offsets within a tile's rows
 bool int8_aligned(const void* q, int64_t ld) {  // 16-byte loads
   return (reinterpret_cast<uintptr_t>(q) | (uint64_t)ld) % 16 == 0 && ld < kInt8Ld;
@@ -441,25 +445,34 @@ Int8Plan int8_plan(const Int8Args& a) {
   const int64_t packed = (ax ? 0 : a.M) + (aw ? 0 : a.N);  // rows to copy
   const double pack_us = packed ? 3 + 2 * packed * k / 5e6 : 0;
   const int64_t pack_bytes = (packed * lda + 255) / 256 * 256;
-  // 16 or 32 rows of x; unaligned rows as they are, or copied first (16 x 4096 x 4099: 8.5 / 20 us, 40 x 64 x 20001: 28 / 16)
+  // 16 or 32 rows of x; unaligned rows as they are, or copied first (16 x 4096 x 4099: 8.5 / 20 us, 40 x 64 x 20001:
+  // 28 / 16); K whole, or in runs of whole steps where there are few tiles (1 x 512 x 25088: 12.6 / 10.1 us, 15 x 64 x
+  // 21419: 16.4 / 12.4)
   for (int s = 0; s < 4; ++s) {
     if (s >= 2 && aligned) break;
     if (s < 2 && (a.ldw >= kInt8Ld || a.ldx >= kInt8Ld)) continue;
-    Int8Plan p = {};
-    p.kind = s & 1;
-    p.pack = s >= 2;
-    p.lda = lda;
-    p.nt = div_up(a.N, 16);
-    p.mt = div_up(a.M, 16 << p.kind);
-    p.splits = 1;
-    const double blocks = (double)p.nt * p.mt, rows = std::min<double>(a.M, 16 << p.kind);
-    p.us = std::max(hbm, std::ceil(blocks / 512) * (std::ceil(nk / 16.0) * (aligned || p.pack ? 0.9 : 1.3) + 2)) +
-           blocks * (rows + (p.mt > 1 ? 16 : 0)) * k / 12e6 + 2;
-    if (p.pack) {
-      p.us += pack_us;
-      p.pack_bytes = p.bytes = pack_bytes;
+    for (int splits : {1, 2, 3, 4, 6, 8, 12}) {
+      Int8Plan p = {};
+      p.kind = s & 1;
+      p.pack = s >= 2;
+      p.lda = lda;
+      p.nt = div_up(a.N, 16);
+      p.mt = div_up(a.M, 16 << p.kind);
+      const int run = div_up(div_up(nk, splits), kStreamTiles) * kStreamTiles;
+      p.run = run * 128;
+      p.splits = div_up(nk, run);
+      if (p.splits != splits) continue;
+      const double blocks = (double)p.nt * p.mt * splits, rows = std::min<double>(a.M, 16 << p.kind);
+      p.us = std::max(hbm, std::ceil(blocks / 512) * (run / kStreamTiles * (aligned || p.pack ? 0.9 : 2.2) + 2)) +
+             blocks / splits * (rows + (p.mt > 1 ? 16 : 0)) * k / 12e6 + 2;
+      if (splits > 1) p.us += 5 + splits * mn * 8 / 6e6;
+      if (p.pack) {
+        p.us += pack_us;
+        p.pack_bytes = pack_bytes;
+      }
+      p.bytes = p.pack_bytes + (splits > 1 ? splits * a.M * a.N * 4 : 0);
+      if (blocks < kInt8Blocks && p.us < best.us) best = p;
     }
-    if (blocks < kInt8Blocks && p.us < best.us) best = p;
   }
   for (int t = 0; t < 3; ++t) {
     const Int8Cand& c = kInt8Tiles[t];
@@ -527,17 +540,16 @@ void int8_matmul(const Int8Args& args, void* ws, hipStream_t st) {
     }
     a.K = p.lda;
   }
-  if (p.kind < 2) {
-    const bool aligned = int8_x_aligned(a) && int8_w_aligned(a);
-    const unsigned grid = (unsigned)(p.nt * p.mt);
-    if (p.kind == 0 && aligned) int8_stream_kernel<1, true><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
-    else if (p.kind == 0) int8_stream_kernel<1, false><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
-    else if (aligned) int8_stream_kernel<2, true><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
-    else int8_stream_kernel<2, false><<<grid, 512, 0, st>>>(a, p.nt, p.mt);
-    return;
-  }
   int32_t* part = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + p.pack_bytes);
-  if (p.kind == 2) int8_tiles<Int8Tile64>(a, p, part, st);
+  const auto stream = [&](auto kernel) {
+    kernel<<<(unsigned)(p.nt * p.mt * p.splits), 512, 0, st>>>(a, p.nt, p.mt, p.splits, p.run, part);
+  };
+  const bool aligned = int8_x_aligned(a) && int8_w_aligned(a);
+  if (p.kind == 0 && aligned) stream(int8_stream_kernel<1, true>);
+  else if (p.kind == 0) stream(int8_stream_kernel<1, false>);
+  else if (p.kind == 1 && aligned) stream(int8_stream_kernel<2, true>);
+  else if (p.kind == 1) stream(int8_stream_kernel<2, false>);
+  else if (p.kind == 2) int8_tiles<Int8Tile64>(a, p, part, st);
   else if (p.kind == 3) int8_tiles<Int8Tile128>(a, p, part, st);
   else int8_tiles<Int8Tile256>(a, p, part, st);
   if (p.splits > 1)

@@ -758,8 +758,8 @@ double ns_cut(NsGroup* g, int ng, int cap) {
   return any ? 5 + bytes / 4.5e6 : 0;
 }
 
-// The tile of X X^T and the runs of its K.  Whole / cut, us in all: 64 x 4608 144 / 90, 512 x 4608 276 / 231, VGG16's update
-// 17250 / 16900; for ResNet-101's matrices 126 / 90 + 16 in this launch (uncut, 80 are one tile of 512 x 9216).
+// The tile of X X^T and the runs of its K.  Whole / cut, us in all: 64 x 4608 144 / 90, 512 x 4608 276 / 231, VGG16's
+// update 17250 / 16900; for ResNet-101's matrices 126 / 90 + 16 in this launch (uncut, 80 are one tile of 512 x 9216).
 int ns_pick_gram(NsGroup* g, int ng, bool& cut) {
   constexpr int kWhole = 1 << 20;
   int tile = 0, runs = kWhole;

@@ -240,7 +240,8 @@ __device__ __forceinline__ void nt_loop_body(char* lds, const char* __restrict__
                              : kNtOob;
     } else {
       chunk[i] += g * 128;
-      off[i] = g < C::KG && row < (is_b ? brows : arows) ? (uint32_t)row * (is_b ? B.ld : A.ld) + (uint32_t)chunk[i] : kNtOob;
+      off[i] = g < C::KG && row < (is_b ? brows : arows) ? (uint32_t)row * (is_b ? B.ld : A.ld) + (uint32_t)chunk[i]
+                                                         : kNtOob;
     }
   }
   // int8: one window per operand, up to the end of its last row

@@ -170,6 +170,18 @@ def test_int8_matmul_any_address(cuda, M, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('M,N,K', [(1, 512, 25088), (15, 64, 21419), (20, 530, 7026), (40, 64, 20001), (33, 20, 30000),
+                                   (16, 33, 16385), (2, 70, 131071)])
+def test_int8_matmul_long_rows(cuda, M, N, K):
+    """Few rows and a long K, which is cut into runs: the sums stay exact."""
+    gen = torch.Generator().manual_seed(K)
+    x, w = (torch.randint(-128, 128, (r, K), generator=gen).to(torch.int8) for r in (M, N))
+    one = torch.ones(max(M, N), device=cuda)
+    got = ops.int8_matmul(x.to(cuda), one[:M], w.to(cuda), one[:N], out_dtype=torch.float32)
+    assert torch.equal(got.cpu(), (x.to(torch.int64) @ w.to(torch.int64).t()).float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('K', [5, 9, 100])
 def test_more_rows_than_one_launch_takes(cuda, K):
     """Rows past 2^21 (quantized, copied) and 2^22 blocks: the last ones are as if they were alone."""
