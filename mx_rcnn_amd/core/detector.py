@@ -61,7 +61,8 @@ def _inference_copy(model, dtype):
 
 def _quantize_fc(model, source):
     """The FC layers ahead of the predictors (VGG16's fc6 / fc7) of the inference copy ``model`` in 8 bits,
-    from ``source``'s weights: int8 rows with one scale per output channel, laid out once (ops/int8.py)."""
+    from ``source``'s weights: int8 rows with one scale per output channel, laid out once (ops/int8.py).  Nothing
+    of ``source`` is shared: it may train on while the detector keeps what it was built with."""
     from ..ops.int8 import quantize_rows
     names = [k for k in ('fc6', 'fc7') if hasattr(model.head, k)]
     if not names:
@@ -70,7 +71,7 @@ def _quantize_fc(model, source):
         for k in names:
             layer, w = getattr(model.head, k), getattr(source.head, k).weight.detach().float()
             layer.int8 = quantize_rows(layer.rows_of(w).contiguous()) + \
-                (None if layer.bias is None else getattr(source.head, k).bias.detach().float(),)
+                (None if layer.bias is None else getattr(source.head, k).bias.detach().float().clone(),)
 
 
 class Detector(object):
