@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void*
 #pragma unroll
       for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(v[c].get(e)));
   } else {
-    for (int k = tid * 8; k < K; k += T * 8) {
-      v[0].load(x, x0 + min(k, K - 8));
+    for (int64_t k = tid * 8; k < K; k += T * 8) {  // (64 bits: K reaches 2^31 - 1)
+      v[0].load(x, x0 + min(k, (int64_t)K - 8));
 #pragma unroll
       for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(v[0].get(e)));
     }
@@ -115,17 +115,17 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_kernel(const void*
     scale[row] = s;
     for (int k = K; k < ldq; ++k) out[k] = 0;
   }
-  const auto put = [&](const Raw8<CODE>& d, int k) {
+  const auto put = [&](const Raw8<CODE>& d, int64_t k) {
     const uint2 w = bad ? make_uint2(0, 0) : to_i8x8(d, s, inv);
-    __builtin_memcpy(out + min(k, K - 8), &w, 8);
+    __builtin_memcpy(out + min(k, (int64_t)K - 8), &w, 8);
   };
   if constexpr (HELD) {
 #pragma unroll
     for (int c = 0; c < NV; ++c)
       if ((c * T + tid) * 8 < K) put(v[c], (c * T + tid) * 8);
   } else {
-    for (int k = tid * 8; k < K; k += T * 8) {
-      v[0].load(x, x0 + min(k, K - 8));
+    for (int64_t k = tid * 8; k < K; k += T * 8) {
+      v[0].load(x, x0 + min(k, (int64_t)K - 8));
       put(v[0], k);
     }
   }
