@@ -87,10 +87,11 @@ __device__ __forceinline__ void st4_pair(uint16_t* d, const float v[4]) {  // 4 
 }
 
 // ---- the values that are orthogonalised ---------------------------------------------------------
-// u = G, or for the update g' = clip(rescale g), mom' = mu mom + g', u = g' + mu mom' (nesterov) or mom'
-__device__ __forceinline__ float ns_grad(const NsUpdate& u, int64_t i) {
-  float g = ld(u.grad, i, u.code) * u.rescale;
-  if (u.clip > 0.f) g = fminf(fmaxf(g, -u.clip), u.clip);
+// u = G, or for the update g' = clip(rescale g), mom' = mu mom + g', u = g' + mu mom' (nesterov) or mom'.
+// A NaN passes the clip (fminf / fmaxf would make it -clip and hide it).
+__device__ __forceinline__ float ns_clip(const NsUpdate& u, float g) {
+  g *= u.rescale;
+  if (u.clip > 0.f) g = g < -u.clip ? -u.clip : g > u.clip ? u.clip : g;
   return g;
 }
 
@@ -123,8 +124,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs p, NsUpdate u) {
       ns_ld4(u.mom, off + i, 0, vec && cnt == 4, cnt, m);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float gv = v[e] * u.rescale;
-        if (u.clip > 0.f) gv = fminf(fmaxf(gv, -u.clip), u.clip);
+        const float gv = ns_clip(u, v[e]);
         m[e] = u.mu * m[e] + gv;
         v[e] = u.nesterov ? gv + u.mu * m[e] : m[e];
       }
@@ -181,8 +181,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
         ns_ld4(u.mom, i, 0, vec, cnt, m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float gv = v[e] * u.rescale;
-          if (u.clip > 0.f) gv = fminf(fmaxf(gv, -u.clip), u.clip);
+          const float gv = ns_clip(u, v[e]);
           v[e] = u.nesterov ? gv + u.mu * m[e] : m[e];
         }
       }
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(1024) ns_block_kernel(NsArgs p, NsUpdate u, in
   };
   double s = 0.0;
   for (int i = tid; i < total; i += 1024) {
-    float v = ns_grad(u, off + i);
+    float v = ns_clip(u, ld(u.grad, off + i, u.code));
     if (u.mom != nullptr) {
       const float m = u.mu * u.mom[off + i] + v;
       u.mom[off + i] = m;

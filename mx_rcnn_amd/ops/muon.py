@@ -76,6 +76,7 @@ def muon_update_(w, mom, grad, mats, lr, momentum=0.95, wd=0.0, rescale=1.0, cli
         g = clip(rescale * grad),  mom = momentum * mom + g,  u = g + momentum * mom (nesterov) or mom
         w -= lr * (sqrt(max(1, rows / cols)) * orthogonalize(u) + wd * w)
 
+    A NaN in a matrix's gradient is not clipped away: that matrix's weights become NaN, the others' do not.
     ``lr``, ``w_bf16``, ``planes``, ``plane_stride`` and ``zero`` are those of :func:`sgd_momentum_`: a
     1-element fp32 device tensor, the low-precision copy of the new weights, its planes, and the gradient
     buffer to clear once read (the matrices' elements of it).  All matrices of a call share its launches, and
