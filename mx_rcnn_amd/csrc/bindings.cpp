@@ -774,11 +774,10 @@ void muon_update(Tensor w, Tensor mom, const Tensor& grad, const std::vector<std
     u.shadow_plane = stride;
   }
   if (zero.has_value() && zero->defined()) {
-    TORCH_CHECK(zero->is_contiguous() && zero->numel() == w.numel() && zero->device() == w.device() &&
-                    (zero->scalar_type() == at::kFloat || zero->scalar_type() == at::kBFloat16),
-                "zero: contiguous fp32 / bf16 of numel elements");
+    TORCH_CHECK(zero->is_contiguous() && zero->numel() == w.numel() && zero->device() == w.device(),
+                "zero: contiguous fp32, bf16 or fp16 of numel elements on the weights' device");
     u.zero = zero->data_ptr();
-    u.zero_code = is_bf16(*zero);
+    u.zero_code = ns_code(*zero, "muon_update zero");
   }
   if (mats.empty()) return;
   DevGuard g(w.device());
