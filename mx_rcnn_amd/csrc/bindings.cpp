@@ -654,6 +654,13 @@ static int ns_code(const Tensor& t, const char* what) {
               ": fp32, bf16 or fp16, not ", t.scalar_type());
   return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2;
 }
+// an operator without a backward pass must not drop a gradient that the caller records
+static void refuse_grad(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!(t->defined() && t->requires_grad()), what,
+                " is not differentiable: call it under torch.no_grad() or on detached tensors");
+}
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Matrices {element offset, rows, cols} -> launches: groups of equal shape (in order of first appearance), at most
@@ -718,6 +725,7 @@ static void ns_check_shape(int64_t rows, int64_t cols) {
 // (b, r, c) contiguous -> its matrices orthogonalised, same type
 Tensor ns_orthogonalize(const Tensor& g, int64_t steps, double eps) {
   CHECK_DEV(g); CHECK_CONTIG(g);
+  refuse_grad("orthogonalize", {&g});
   TORCH_CHECK(g.dim() == 3, "orthogonalize: (b, r, c)");
   TORCH_CHECK(steps >= 1 && steps <= 16, "orthogonalize: 1 to 16 steps");
   TORCH_CHECK(eps > 0, "orthogonalize: eps must be positive");
@@ -798,6 +806,7 @@ void muon_update(Tensor w, Tensor mom, const Tensor& grad, const std::vector<std
 // ---- 8-bit rows and products (int8_gemm.hip) ----------------------------------------------
 std::vector<Tensor> quantize_rows(const Tensor& x) {
   CHECK_DEV(x);
+  refuse_grad("quantize_rows", {&x});
   TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "quantize_rows: (M, K) with K contiguous");
   const int code = ns_code(x, "quantize_rows");
   TORCH_CHECK(x.size(1) <= INT32_MAX && x.size(0) <= INT32_MAX, "quantize_rows: too large");
@@ -830,9 +839,11 @@ static mxr::Int8Args int8_args(const Tensor& x, const Tensor& w, const Tensor& w
   TORCH_CHECK(w.device() == x.device(), "int8_matmul: operands on different devices");
   TORCH_CHECK(code >= 0 && code <= 2, "int8_matmul: output type");
   check_row_vec(ws, N, x, "ws");
+  refuse_grad("an 8-bit product", {&x, &ws});
   mxr::Int8Args a = {};
   if (bias.has_value() && bias->defined()) {
     check_row_vec(*bias, N, x, "bias");
+    refuse_grad("an 8-bit product", {&*bias});
     a.bias = bias->data_ptr<float>();
   }
   a.w = w.data_ptr<int8_t>();
@@ -864,6 +875,7 @@ Tensor int8_matmul(const Tensor& x, const Tensor& xs, const Tensor& w, const Ten
               "int8_matmul: x is int8 (M, K) with K contiguous");
   mxr::Int8Args a = int8_args(x, w, ws, bias, relu, code);
   check_row_vec(xs, a.M, x, "xs");
+  refuse_grad("an 8-bit product", {&xs});
   DevGuard g(x.device());
   a.x = x.data_ptr<int8_t>();
   a.ldx = x.stride(0);

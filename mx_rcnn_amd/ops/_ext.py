@@ -34,6 +34,14 @@ def _load():
     return _EXT
 
 
+def refuse_grad(what, *tensors):
+    """Raise where an operator without a backward pass would drop the gradient of one of ``tensors``
+    (CPU paths; the extension's entry points have the same check)."""
+    import torch
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError('%s is not differentiable: call it under torch.no_grad() or on detached tensors' % what)
+
+
 def ext_available():
     return _load() is not None
 

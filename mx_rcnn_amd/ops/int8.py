@@ -5,11 +5,13 @@ A fully connected layer in this form keeps its weight as ``quantize_rows(weight)
 output channel, laid out once -- and quantizes its input rows (one scale per RoI) in each call.  VGG16's
 fc6 then reads 103 MB of weights instead of 205 MB of bf16, at twice the matrix-core rate.
 
+None of them is differentiable: an input that records a gradient is refused.
+
 CPU tensors run the PyTorch form below, which is also the oracle of the kernels.
 """
 import torch
 
-from ._ext import need_ext
+from ._ext import need_ext, refuse_grad
 
 TINY = 2.0 ** -126
 MAX_K = 131071  # int32 sums of 8-bit products are exact up to here, -128 included
@@ -27,6 +29,7 @@ def quantize_rows(x):
     A row that holds an infinity or a NaN gets the scale NaN and zeros: what is computed from it is NaN."""
     if x.is_cuda:
         return tuple(need_ext().quantize_rows(_rows(x)))
+    refuse_grad('quantize_rows', x)
     _check_float(x, 'quantize_rows')
     if x.dim() != 2:
         raise ValueError('quantize_rows: (M, K), not %s' % (tuple(x.shape),))
@@ -55,6 +58,7 @@ def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16)
         raise ValueError('int8_matmul: K = %d (int32 sums are exact up to %d)' % (xq.shape[1], MAX_K))
     if xq.is_cuda:  # (the extension checks the rest)
         return need_ext().int8_matmul(_rows(xq), xs, _rows(wq), ws, bias, relu, OUT_CODES[out_dtype])
+    refuse_grad('int8_matmul', xs, ws, bias)
     for t, what in ((xq, 'xq'), (wq, 'wq')):
         if t.dtype != torch.int8 or t.dim() != 2:
             raise TypeError('int8_matmul: %s must be a 2-D int8 tensor, not %s %s' % (what, t.dtype, tuple(t.shape)))
@@ -77,10 +81,11 @@ def int8_matmul(xq, xs, wq, ws, bias=None, relu=False, out_dtype=torch.bfloat16)
 
 def int8_linear(x, wq, ws, bias=None, relu=False):
     """A fully connected layer on floating rows ``x`` (M, K) with an 8-bit weight (``quantize_rows`` of the
-    (N, K) weight): the rows quantized, multiplied, scaled back; result in x's type.  Not differentiable."""
+    (N, K) weight): the rows quantized, multiplied, scaled back; result in x's type."""
     if x.is_cuda:  # one call; the rows are quantized into the layout that the product reads
         if x.dim() == 2 and x.shape[1] > MAX_K:
             raise ValueError('int8_linear: K = %d (int32 sums are exact up to %d)' % (x.shape[1], MAX_K))
-        return need_ext().int8_linear(_rows(x.detach()), _rows(wq), ws, bias, relu)
-    xq, xs = quantize_rows(x.detach())
+        return need_ext().int8_linear(_rows(x), _rows(wq), ws, bias, relu)
+    refuse_grad('int8_linear', x, ws, bias)
+    xq, xs = quantize_rows(x)
     return int8_matmul(xq, xs, wq, ws, bias, relu, x.dtype)

@@ -12,7 +12,7 @@ import math
 
 import torch
 
-from ._ext import need_ext
+from ._ext import need_ext, refuse_grad
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 EPS = 1e-7
@@ -52,19 +52,20 @@ def orthogonalize(g, steps=5, eps=EPS):
     between about 0.7 and 1.2 after five steps, those far below |G|_F / 500 left smaller).  A matrix of zeros stays
     zero; one that holds an infinity or a NaN comes back as NaN.  Computed in 22-bit operands with fp32 sums
     whatever the type; where |G|_F is far below ``eps``, to an absolute accuracy of about 1e-9.  Not
-    differentiable."""
+    differentiable: an input that records a gradient is refused."""
     if g.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError('orthogonalize: fp32, bf16 or fp16, not %s' % g.dtype)
     if g.dim() not in (2, 3):
         raise ValueError('orthogonalize: (r, c) or (b, r, c), not %s' % (tuple(g.shape),))
     _check_steps(steps, eps)
-    x = g.detach().contiguous()
+    x = g.contiguous()
     x = x.unsqueeze(0) if g.dim() == 2 else x
     if x.numel() == 0:
         return torch.empty_like(x).reshape(g.shape)
     _check_sides(x.shape[1], x.shape[2])
     if x.is_cuda:
         return need_ext().ns_orthogonalize(x, int(steps), float(eps)).reshape(g.shape)
+    refuse_grad('orthogonalize', g)
     return newton_schulz_ref(x.float(), steps, eps).reshape(g.shape).to(g.dtype)
 
 
