@@ -95,6 +95,13 @@ __device__ __forceinline__ float ns_clip(const NsUpdate& u, float g) {
   return g;
 }
 
+// 1 / (|u| + eps).  Finite also where |u| is zero and eps below 1 / DBL_MAX, so that zeros stay zero: any other |u| of
+// fp32 values is at least 2^-149.
+__device__ __forceinline__ double ns_inverse(double squares, double eps) {
+  const double norm = sqrt(squares) + eps;
+  return norm < 1e-300 ? 1e300 : 1.0 / norm;  // (NaN: NaN)
+}
+
 __device__ __forceinline__ void ns_ld4(const void* p, int64_t i, int code, bool vec, int n, float v[4]) {
   if (vec) {
     ld4c(p, i, code, 0, v);
@@ -163,7 +170,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(NsArgs p, NsUpdate u) {
   __shared__ float tile[64][65];
   if ((tid & 63) == 0) red[tid >> 6] = s;
   __syncthreads();
-  const double f = (double)kNsX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + u.eps);
+  const double f = ns_inverse((red[0] + red[1]) + (red[2] + red[3]), u.eps) * (double)kNsX;
   const int lr = tid >> 4, lc = (tid & 15) * 4;
   uint16_t* x = ns_x(p, g, mi, 0);
   // elements as they lie in memory: 4 columns of rows lr, lr + 16, ..
@@ -531,7 +538,7 @@ __global__ void __launch_bounds__(1024) ns_block_kernel(NsArgs p, NsUpdate u, in
   s = 0.0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) s += red[w];
-  const double f = 1.0 / (sqrt(s) + u.eps);
+  const double f = ns_inverse(s, u.eps);
   for (int i = tid; i < pm * lx; i += 1024) X[i] = (float)((double)X[i] * f);
   __syncthreads();
 
