@@ -4,12 +4,14 @@ Explicit hipcc pipeline (no hipify, no JIT cache): every ``hip/*.hip`` is compil
 ``hipcc --offload-arch=gfx950`` into a PIC object, ``bindings.cpp`` (host-only glue)
 with the host compiler against the PyTorch headers, and everything is linked into one
 shared object next to the package so it travels with the repo snapshot to the GPU box.
-Incremental: an object is rebuilt only when its source or a header is newer.
+Incremental: an object is kept only while what it was made from -- compile command, compiler, source and in-tree headers,
+by content -- is unchanged (``<object>.made``), so a changed flag or an older file checked out over a newer one rebuilds.
 
 Usage: ``python -m mx_rcnn_amd.csrc.build [--force] [--jobs N] [--debug]``
 """
 import argparse
 import glob
+import hashlib
 import os
 import re
 import subprocess
@@ -40,11 +42,34 @@ def ext_path():
     return os.path.join(PKG, '_C' + suffix)
 
 
-def _newer(src_list, target):
-    if not os.path.exists(target):
-        return True
-    t = os.path.getmtime(target)
-    return any(os.path.getmtime(s) > t for s in src_list)
+def _made_from(parts, files):
+    """Digest of texts and of files' contents."""
+    h = hashlib.sha256()
+    for p in parts:
+        h.update(p.encode() + b'\0')
+    for f in files:
+        with open(f, 'rb') as fh:
+            h.update(hashlib.sha256(fh.read()).digest())
+    return h.hexdigest()
+
+
+def _record(target):
+    """What ``target`` was made from, or None."""
+    try:
+        with open(target + '.made') as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _forget(target):
+    if os.path.exists(target + '.made'):
+        os.remove(target + '.made')
+
+
+def _remember(target, digest):
+    with open(target + '.made', 'w') as f:
+        f.write(digest)
 
 
 def _run(cmd):
@@ -60,7 +85,7 @@ _INC = re.compile(r'^\s*#\s*include\s+"([^"]+)"', re.M)
 def _local_deps(src, seen=None):
     """The in-tree headers ``src`` includes, transitively (quoted includes resolved next to the
     including file, then in csrc/ and csrc/hip/): an object rebuilds only when one of ITS headers
-    changes (a conv-body edit no longer rebuilds every kernel file)."""
+    changes (a conv-body edit does not rebuild every kernel file)."""
     seen = set() if seen is None else seen
     try:
         text = open(src).read()
@@ -88,35 +113,52 @@ def build(force=False, jobs=None, debug=False, verbose=False):
                        '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, '-I', HERE, '-I', os.path.join(HERE, 'hip')]
     if os.environ.get('MXR_SYNC_DEBUG'):
         hip_flags.append('-DMXR_SYNC_DEBUG=1')
-    jobs_list = []
+    jobs_list = []  # (object, digest, command)
     objs = []
+
+    def add(src, obj, versions, cmd):
+        objs.append(obj)
+        digest = _made_from(versions + cmd, [src] + sorted(_local_deps(src)))
+        if force or not os.path.exists(obj) or _record(obj) != digest:
+            jobs_list.append((obj, digest, cmd))
+
+    hip_versions = [_run([hipcc, '--version'])]
     for src in sorted(glob.glob(os.path.join(HERE, 'hip', '*.hip'))):
         obj = os.path.join(BUILD, os.path.basename(src) + '.o')
-        objs.append(obj)
-        if force or _newer([src] + sorted(_local_deps(src)), obj):
-            jobs_list.append([hipcc] + hip_flags + ['-c', src, '-o', obj])
+        add(src, obj, hip_versions, [hipcc] + hip_flags + ['-c', src, '-o', obj])
     py_inc = sysconfig.get_paths()['include']
     glue = os.path.join(HERE, 'bindings.cpp')
     glue_obj = os.path.join(BUILD, 'bindings.o')
-    objs.append(glue_obj)
-    if force or _newer([glue] + sorted(_local_deps(glue)), glue_obj):
-        cxx = os.environ.get('CXX', 'g++')
-        flags = opt + ['-fPIC', '-std=c++17', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
-                       '-DTORCH_EXTENSION_NAME=_C', '-DTORCH_API_INCLUDE_EXTENSION_H',
-                       '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, '-I', HERE, '-I', os.path.join(ROCM, 'include'),
-                       '-I', py_inc] + sum([['-I', p] for p in tinc], []) + ['-w']
-        jobs_list.append([cxx] + flags + ['-c', glue, '-o', glue_obj])
+    cxx = os.environ.get('CXX', 'g++')
+    flags = opt + ['-fPIC', '-std=c++17', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+                   '-DTORCH_EXTENSION_NAME=_C', '-DTORCH_API_INCLUDE_EXTENSION_H',
+                   '-D_GLIBCXX_USE_CXX11_ABI=%d' % abi, '-I', HERE, '-I', os.path.join(ROCM, 'include'),
+                   '-I', py_inc] + sum([['-I', p] for p in tinc], []) + ['-w']
+    import torch
+    add(glue, glue_obj, [torch.__version__, _run([cxx, '--version'])], [cxx] + flags + ['-c', glue, '-o', glue_obj])
+
+    def compile_one(job):
+        obj, digest, cmd = job
+        _forget(obj)  # (a step that fails or is killed leaves nothing that counts as made)
+        out = _run(cmd)
+        _remember(obj, digest)
+        return out
+
     n = jobs or min(8, max(1, len(jobs_list)))
     with ThreadPoolExecutor(n) as ex:
-        for out in ex.map(_run, jobs_list):
+        for out in ex.map(compile_one, jobs_list):
             if verbose and out.strip():
                 print(out)
     target = ext_path()
-    if force or jobs_list or not os.path.exists(target) or _newer(objs, target):
-        link = ['g++', '-shared', '-o', target] + objs + [
-            '-L', tlib, '-Wl,-rpath,' + tlib, '-lc10', '-lc10_hip', '-ltorch', '-ltorch_cpu', '-ltorch_hip',
-            '-ltorch_python', '-lamdhip64']
+    link = ['g++', '-shared', '-o', target] + objs + [
+        '-L', tlib, '-Wl,-rpath,' + tlib, '-lc10', '-lc10_hip', '-ltorch', '-ltorch_cpu', '-ltorch_hip',
+        '-ltorch_python', '-lamdhip64']
+    made = os.path.join(BUILD, os.path.basename(target))  # (its record stays with the objects')
+    digest = _made_from(link, objs)
+    if force or jobs_list or not os.path.exists(target) or _record(made) != digest + _made_from([], [target]):
+        _forget(made)
         _run(link)
+        _remember(made, digest + _made_from([], [target]))
     return target
 
 
