@@ -742,9 +742,16 @@ double ns_cost(const NsGroup* g, int ng, const NsTile& c, NsLaunch what) {
   return us;
 }
 
+// The 256 tile has no registers for sums in runs, so it takes no sums of squares (X X^T, A A) longer than that many K
+// tiles.  With / without them, error against 64 bits and ms: 12288 x 12288 6.5e-6 89 / 3.5e-6 101, 16384 x 16384 8.9e-6
+// 221 / 4.0e-6 253 (the plain recurrence in fp32 3.4e-6 and 3.6e-6).
+constexpr int kNsLongestSum = 160;
+
 int ns_pick(const NsGroup* g, int ng, NsLaunch what) {
+  int longest = 0;
+  for (int i = 0; i < ng; ++i) longest = std::max(longest, what == kLaunchGram ? g[i].run_k : g[i].mp / 32);
   int best = 0;
-  for (int t = 1; t < 4; ++t)
+  for (int t = 1; t < (longest > kNsLongestSum && what != kLaunchRect ? 3 : 4); ++t)
     if (ns_cost(g, ng, kNsTiles[t], what) < ns_cost(g, ng, kNsTiles[best], what)) best = t;
   return best;
 }
