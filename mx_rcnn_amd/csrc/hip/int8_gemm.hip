@@ -150,9 +150,10 @@ void quantize(const void* x, int64_t rows, int64_t ld, int K, int8_t* q, int ldq
     const int per = t < 256 ? 256 / t : 1;
     kernel<<<(unsigned)((rows + per - 1) / per), t < 256 ? 256 : t, 0, st>>>(x, ld, rows, K, q, ldq, scale);
   };
-  // bf16 rows, us, one way and the next: 2048 x 512 2.7 / 2.9 (a wave, 8 values a lane / 32), 2048 x 1024 3.5 / 4.2
-  // but 64 x 1024 3.1 / 2.7 (a wave / 256 threads), 2048 x 4096 7.3 / 8.1 (256 / 512), 2048 x 8192 11 / 15.5 (16 values / 64),
-  // 2048 x 32768 39 / 50 (held / read twice); 2400 x 25088 with 256 / 512 / 1024 threads per row 36 / 33 / 41 (5.5 TB/s)
+  // bf16 rows (fp32 and fp16 rows follow the same limits, not measured apart), us, one way and the next: 2048 x 512
+  // 2.7 / 2.9 (a wave, 8 values a lane / 32), 2048 x 1024 3.5 / 4.2 but 64 x 1024 3.1 / 2.7 (a wave / 256 threads), 2048 x
+  // 4096 7.3 / 8.1 (256 / 512), 2048 x 8192 11 / 15.5 (16 values / 64), 2048 x 32768 39 / 50 (held / read twice); 2400 x
+  // 25088 with 256 / 512 / 1024 threads per row 36 / 33 / 41 (5.5 TB/s)
   if (K < 8) quantize_short_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(x, CODE, ld, rows, K, q, ldq, scale);
   else if (K <= 512) go(quantize_kernel<CODE, 64, 1, true>, 64);
   else if (K <= 2048 && rows >= 2048) go(quantize_kernel<CODE, 64, 4, true>, 64);
@@ -405,9 +406,9 @@ __global__ void __launch_bounds__(256) int8_join_kernel(Int8Args p, int splits, 
 // ---- choice of kernel ---------------------------------------------------------------------------
 // Tiles and their measured cost: microseconds per K tile of 128 bytes with up to half of the slots (blocks resident on
 // the chip) taken and with all, and per round (start, epilogue).  Runs of K summed apart cost a second launch and
-// their traffic.  Measured, us: 300 x 4096 x 25088 in 4 runs of 128 x 160 tiles 50, in 8 of 256 x 160 56, in 5 of 128 x 128
-// 55, in 8 of 256 x 256 60; 2400 x 4096 x 25088 258 with 256 x 160 (1.9 POPS), 264 256 x 256 (3 runs), 295 128 x 160, 569
-// 64 x 64; 64 x 4096 x 25088 25 in 4 runs of 64 x 64, 28 in 8 of 128 x 160.
+// their traffic.  Measured at these rows only, us: 300 x 4096 x 25088 in 4 runs of 128 x 160 tiles 50, in 8 of 256 x 160
+// 56, in 5 of 128 x 128 55, in 8 of 256 x 256 60; 2400 x 4096 x 25088 258 with 256 x 160 (1.9 POPS), 264 256 x 256 (3
+// runs), 295 128 x 160, 569 64 x 64; 64 x 4096 x 25088 25 in 4 runs of 64 x 64, 28 in 8 of 128 x 160.
 using Int8Tile64 = NtCfg<false, 64, 64, 1, 2, 2, 4>;
 using Int8Tile128 = NtCfg<false, 128, 160, 1, 4, 2, 4>;  // (a ring of 4 fills the LDS)
 using Int8Tile256 = NtCfg<false, 256, 160, 1, 4, 2, 2>;

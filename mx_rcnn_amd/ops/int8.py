@@ -25,8 +25,8 @@ def _check_float(x, what):
 
 def quantize_rows(x):
     """(M, K) fp32 / bf16 / fp16 -> (int8 (M, K), fp32 scales (M,)): scale = max|row| * (1 / 127) in fp32
-    (at least 2^-126), values divided by it and rounded to the nearest integer, ties to even, so that ``q * scale`` stands for the row.
-    A row that holds an infinity or a NaN gets the scale NaN and zeros: what is computed from it is NaN."""
+    (at least 2^-126), values divided by it and rounded to the nearest integer, ties to even, so that ``q * scale`` stands
+    for the row.  A row that holds an infinity or a NaN gets the scale NaN and zeros: what is computed from it is NaN."""
     if x.is_cuda:
         return tuple(need_ext().quantize_rows(_rows(x)))
     refuse_grad('quantize_rows', x)
