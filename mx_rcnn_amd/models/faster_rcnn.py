@@ -14,6 +14,7 @@ proposal target and RoIPool are HIP kernels; no host synchronisation in a traini
 so the whole step can be captured in a hipGraph (core/graph.py).  Images per device may be
 > 1 (the reference is limited to 1: `rcnn/rpn/proposal.py:194`).
 """
+import copy
 import math
 
 import os
@@ -138,18 +139,28 @@ class FasterRCNN(nn.Module):
         """Set the trunk's frozen BN moving statistics from one fp32 forward over ``data`` (N,3,H,W).
         Random-init ResNets have no meaningful frozen statistics; without this their activations
         grow through 100+ pre-activation units.  Pretrained checkpoints carry real ones (load them
-        after, or skip this)."""
-        bns = [m for m in self.trunk.modules() if hasattr(m, 'moving_var')]
-        was = self.training
-        self.eval()
+        after, or skip this).
+
+        Runs on the CPU wherever the model is, like calibrate_vgg: the vendor's fp32 convolutions on the GPU are
+        chosen by timing, differ from process to process, and one of them sums with atomics, so that the same
+        model and data started from other statistics in every run."""
+        trunk = self.trunk
+        if next(trunk.parameters()).is_cuda:
+            trunk = copy.deepcopy(trunk).cpu()
+        bns = [m for m in trunk.modules() if hasattr(m, 'moving_var')]
+        was = trunk.training
+        trunk.eval()
         for m in bns:
             m._calibrate = True
         try:
-            self.trunk(data.float())
+            trunk(data.float().cpu())
         finally:
             for m in bns:
                 m._calibrate = False
-            self.train(was)
+            trunk.train(was)
+        for src, dst in zip(trunk.buffers(), self.trunk.buffers()):
+            if src is not dst:
+                dst.copy_(src)
         return len(bns)
 
     @torch.no_grad()
