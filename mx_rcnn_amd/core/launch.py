@@ -62,7 +62,9 @@ def add_optimizer_args(parser):
     parser.add_argument('--optimizer', default='sgd', choices=('sgd', 'muon'),
                         help='sgd (the reference optimizer) or muon: conv / FC weights except the predictors step '
                              'along their orthogonalised momentum (ops/muon.py), the rest with sgd')
-    parser.add_argument('--muon-lr-mult', dest='muon_lr_mult', type=float, default=20.0,
+    # rates of 0.0004 to 0.002 train random-init ResNet-101 and VGG16 from the first step, 0.005 and more blow up in the
+    # frozen BN's fixed statistics (20 x 0.001 did)
+    parser.add_argument('--muon-lr-mult', dest='muon_lr_mult', type=float, default=0.4,
                         help='learning rate of the muon matrices, as a multiple of --lr')
     return parser
 

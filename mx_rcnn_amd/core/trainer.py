@@ -33,7 +33,9 @@ class Trainer:
 
         optimizer: 'sgd' (the reference's), or 'muon': the conv / FC weights except the predictors step
         along their orthogonalised momentum (ops/muon.py) at ``muon_lr_mult`` times the learning rate with
-        ``muon_momentum``, everything else with SGD as before."""
+        ``muon_momentum``, everything else with SGD as before.  A step moves every direction of a matrix by about
+        that rate: with random-init filters under frozen BN rates above 0.002 diverge (the commands pass 0.4 times
+        theirs), the default of 20 is for filters of spectral norms well above 1."""
         if optimizer not in ('sgd', 'muon'):
             raise ValueError('optimizer must be sgd or muon, not %r' % (optimizer,))
         dev = torch.device(device) if device is not None else next(model.parameters()).device
