@@ -291,8 +291,8 @@ class MutableModule(object):
                 h = torch.tensor([float(zlib.crc32(repr(sync_key(key)).encode()))], dtype=torch.float64,
                                  device=self.context)
                 lo, hi = h.clone(), h.clone()
-                torch.distributed.all_reduce(lo, op=torch.distributed.ReduceOp.MIN)
-                torch.distributed.all_reduce(hi, op=torch.distributed.ReduceOp.MAX)
+                pdist.all_reduce(lo, op=torch.distributed.ReduceOp.MIN)
+                pdist.all_reduce(hi, op=torch.distributed.ReduceOp.MAX)
                 if float(lo.item()) != float(hi.item()):
                     raise RuntimeError('ranks reached different input shapes at a capture point (%s); the data '
                                        'loaders must pad every rank to the global step shape' % (key,))

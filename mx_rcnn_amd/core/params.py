@@ -342,18 +342,18 @@ class FlatParamStore:
         checkpoint; random-init or per-rank-calibrated models would otherwise train apart):
         the flat fp32 masters (bf16 shadows re-derived), the frozen parameters and the model
         buffers (BN moving statistics), then the dgrad filter cache."""
-        import torch.distributed as dist
+        from ..parallel.dist import broadcast
         for g in self.groups:
-            dist.broadcast(g.master, src)
+            broadcast(g.master, src)
             g.sync_shadow()
         for n in self.fixed_names:
-            dist.broadcast(self.frozen_fp32[n], src)
+            broadcast(self.frozen_fp32[n], src)
             self.params[n].data.copy_(self.frozen_fp32[n].to(self.params[n].dtype))
             precision.forget_weight(self.params[n])  # .data writes do not move the version counter
         for b in self.model.buffers():
             if b.is_floating_point() or b.dtype in (torch.int32, torch.int64):
                 t = b.data if b.is_contiguous() else b.data.contiguous()
-                dist.broadcast(t, src)
+                broadcast(t, src)
                 if t is not b.data:
                     b.data.copy_(t)
         self.refresh_dgrad_cache()

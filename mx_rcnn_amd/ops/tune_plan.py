@@ -120,6 +120,8 @@ def sync_from_rank0(device=None):
     if not (dist.is_available() and dist.is_initialized()) or dist.get_world_size() == 1:
         return plan_hash(mine)
     box = [mine if dist.get_rank() == 0 else None]
+    if dist.get_backend() == 'gloo':
+        device = None  # (host memory)
     dist.broadcast_object_list(box, src=0, device=device)
     ext.conv_tune_set(box[0], True)
     return plan_hash(box[0])

@@ -86,8 +86,51 @@ def barrier():
             dist.barrier()
 
 
+def _through_host(t):
+    """gloo gets host memory only: device tensors it copies on streams of its own, in which several ranks on one GPU
+    have hung."""
+    return t.is_cuda and dist.get_backend() == 'gloo'
+
+
+class _HostWork(object):
+    """A collective on the host copy of ``t``, brought back by the first ``wait``."""
+
+    def __init__(self, t, host, work):
+        self.t, self.host, self.work = t, host, work
+
+    def wait(self):
+        if self.work is not None:
+            self.work.wait()
+            self.t.copy_(self.host)  # (has arrived on return, for every stream)
+            self.work = self.host = None
+        return True
+
+
+def all_reduce(t, op=dist.ReduceOp.SUM, async_op=False):
+    """dist.all_reduce of ``t``; device tensors go through host memory where gloo carries them."""
+    if not _through_host(t):
+        return dist.all_reduce(t, op=op, async_op=async_op)
+    host = t.detach().to('cpu', copy=True)  # waits for the current stream's work on t
+    work = _HostWork(t, host, dist.all_reduce(host, op=op, async_op=True))
+    if async_op:
+        return work
+    work.wait()
+
+
+def broadcast(t, src):
+    """dist.broadcast of ``t``, the same way."""
+    if not _through_host(t):
+        dist.broadcast(t, src)
+        return
+    host = t.detach().to('cpu', copy=True)
+    dist.broadcast(host, src)
+    t.copy_(host)
+
+
 def all_reduce_max(value, device):
     """Max of a python float across ranks."""
+    if is_distributed() and dist.get_backend() == 'gloo':
+        device = 'cpu'
     t = torch.tensor([float(value)], dtype=torch.float64, device=device)
     if is_distributed():
         dist.all_reduce(t, op=dist.ReduceOp.MAX)

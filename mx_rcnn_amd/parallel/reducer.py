@@ -30,7 +30,7 @@ import torch
 import torch.distributed as dist
 
 from ..ops import grad_sink
-from .dist import get_world_size, is_distributed
+from .dist import all_reduce, get_world_size, is_distributed
 
 
 class _nullctx(object):
@@ -171,7 +171,7 @@ class BucketReducer:
                 w.copy_(t)
                 if self.average:
                     w.div_(self.world)
-                b.work = dist.all_reduce(w, op=dist.ReduceOp.SUM, async_op=True)
+                b.work = all_reduce(w, op=dist.ReduceOp.SUM, async_op=True)
             return
         if b.comm is not None:
             w = b.comm[b.start:b.end]
@@ -179,7 +179,7 @@ class BucketReducer:
             t = w
         if self.average:
             t.div_(self.world)
-        b.work = dist.all_reduce(t, op=dist.ReduceOp.SUM, async_op=True)
+        b.work = all_reduce(t, op=dist.ReduceOp.SUM, async_op=True)
 
     def _update(self, b):
         """SGD of one final bucket on the optimizer stream (after its all-reduce under DP; the CPU
@@ -264,25 +264,25 @@ class BucketReducer:
         out_ms = []
         for t in tensors:
             for _ in range(warmup):
-                dist.all_reduce(t)
+                all_reduce(t)
             if cuda:
                 ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 torch.cuda.synchronize()
                 ev0.record()
                 for _ in range(iters):
-                    dist.all_reduce(t)
+                    all_reduce(t)
                 ev1.record()
                 ev1.synchronize()
                 ms = ev0.elapsed_time(ev1) / iters
             else:
                 t0 = time.perf_counter()
                 for _ in range(iters):
-                    dist.all_reduce(t)
+                    all_reduce(t)
                 ms = (time.perf_counter() - t0) * 1e3 / iters
             out_ms.append(ms)
         # the slowest rank defines the collective time
         agg = torch.tensor(out_ms, dtype=torch.float64, device=self.store.device)
-        dist.all_reduce(agg, op=dist.ReduceOp.MAX)
+        all_reduce(agg, op=dist.ReduceOp.MAX)
         out_ms = [float(v) for v in agg.tolist()]
         nbytes = self.bucket_sizes()
         total = sum(out_ms)
